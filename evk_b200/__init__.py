@@ -27,6 +27,13 @@ MM_TRANSPOSE_B = 2
 MM_ACC_C = 4
 ATTN_CAUSAL = 1
 ATTN_BWD_NORMALIZED = 2
+ACT_NONE = 0
+ACT_RELU = 1
+ACT_GELU = 2
+ACT_SILU = 3
+QK_HALF_SPLIT = 1
+QK_CACHE = 2
+QK_ACC_GAIN = 4
 
 STATUS = {
     0: "OK",
@@ -424,6 +431,245 @@ def flash_attention_bwd(q, k, v, o, dO, dQ, dK, dV, heads: Optional[int] = None,
         _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(dO), _ptr(dQ), _ptr(dK), _ptr(dV), B, N, H, Hkv, Dh, scale, flags,
         _dtype_code(q), _stream(stream)))
     return dQ, dK, dV
+
+
+# ------------------------------------- decoder-layer operators (extension) --
+class QkNormRopeDesc(ctypes.Structure):
+    """evkcu_qk_norm_rope_desc (include/evkcu.h)."""
+
+    _fields_ = [(n, ctypes.c_uint32) for n in ("batch", "seq_len", "heads", "kv_heads", "head_dim", "rot_dim", "flags",
+                                                "pos_offset", "cache_len")] + \
+               [("eps", ctypes.c_float), ("base", ctypes.c_float), ("positions", ctypes.c_void_p)] + \
+               [(n, ctypes.c_uint64) for n in ("q_pitch", "k_pitch", "v_pitch", "q_out_pitch", "k_out_pitch",
+                                                "dq_pitch", "dk_pitch")]
+
+
+SIGNATURES.update({
+    "evkcu_linear": [_vp] * 6 + [_u32, _u32, _u32, _int, _u32, _int, _vp],
+    "evkcu_linear_backward": [_vp] * 8 + [_u32, _u32, _u32, _int, _u32, _int, _vp],
+    "evkcu_gated_ffn": [_vp] * 7 + [_u32, _u32, _u32, _int, _u32, _int, _vp],
+    "evkcu_gated_ffn_backward": [_vp] * 10 + [_u32, _u32, _u32, _int, _u32, _int, _vp],
+    "evkcu_qk_norm_rope": [ctypes.POINTER(QkNormRopeDesc)] + [_vp] * 8 + [_int, _vp],
+    "evkcu_qk_norm_rope_backward": [ctypes.POINTER(QkNormRopeDesc)] + [_vp] * 11 + [_u64, _int, _vp],
+    "evkcu_qk_norm_rope_workspace": [_u32],
+})
+_RET["evkcu_qk_norm_rope_workspace"] = _u64
+
+
+def _same(op, like, shapes):
+    """Checks tensors (None allowed) against `like`'s dtype and device and the
+    wanted shapes: {name: (tensor, shape)}."""
+    import torch
+
+    if like.is_cuda and like.get_device() != torch.cuda.current_device():
+        raise EvkcuError(op, 7, f"tensors are on cuda:{like.get_device()}, the current device is "
+                                f"cuda:{torch.cuda.current_device()}")
+    for name, (t, shape) in shapes.items():
+        if t is None:
+            continue
+        if t.dtype != like.dtype or t.device != like.device:
+            raise EvkcuError(op, 7, f"{name} is {t.dtype} on {t.device}, expected {like.dtype} on {like.device}")
+        if tuple(t.shape) != tuple(shape):
+            raise EvkcuError(op, 1, f"{name} is {tuple(t.shape)}, expected {tuple(shape)}")
+
+
+def linear(x, w, y, bias=None, residual=None, act=ACT_NONE, pre=None, transpose_w=False, stream=None):
+    """y = act(x @ w + bias) + residual (evkcu_linear).
+
+    x (..., K); w (K, N), or (N, K) with transpose_w; bias (N,); residual, y
+    and pre (..., N), pre receiving x @ w + bias for linear_backward.  residual
+    may be y."""
+    K = x.shape[-1]
+    N = y.shape[-1]
+    lead = tuple(x.shape[:-1])
+    out = lead + (N,)
+    _same("linear", x, dict(w=(w, (N, K) if transpose_w else (K, N)), y=(y, out), bias=(bias, (N,)),
+                            residual=(residual, out), pre=(pre, out)))
+    _check("evkcu_linear", lib().evkcu_linear(
+        _ptr(x), _ptr(w), _ptr(bias), _ptr(residual), _ptr(y), _ptr(pre), x.numel() // K if K else 0, K, N, act,
+        MM_TRANSPOSE_B if transpose_w else 0, _dtype_code(x), _stream(stream)))
+    return y
+
+
+def linear_backward(x, w, dy, dx=None, dw=None, dbias=None, act=ACT_NONE, pre=None, dpre=None, transpose_w=False,
+                    acc=False, stream=None):
+    """Gradients of linear from dy (evkcu_linear_backward) into those of dx, dw
+    and dbias that are given; acc adds to them.  With an activation, pre is
+    linear's and dpre (like pre; pre or dy itself is allowed) receives the
+    gradient of x @ w + bias."""
+    K, N = x.shape[-1], dy.shape[-1]
+    out = tuple(x.shape[:-1]) + (N,)
+    wshape = (N, K) if transpose_w else (K, N)
+    _same("linear_backward", x, dict(w=(w, wshape), dy=(dy, out), dx=(dx, x.shape), dw=(dw, wshape),
+                                     dbias=(dbias, (N,)), pre=(pre, out), dpre=(dpre, out)))
+    flags = (MM_TRANSPOSE_B if transpose_w else 0) | (MM_ACC_C if acc else 0)
+    _check("evkcu_linear_backward", lib().evkcu_linear_backward(
+        _ptr(x), _ptr(w), _ptr(pre), _ptr(dy), _ptr(dpre), _ptr(dx), _ptr(dw), _ptr(dbias),
+        x.numel() // K if K else 0, K, N, act, flags, _dtype_code(x), _stream(stream)))
+    return dx, dw, dbias
+
+
+def gated_ffn(x, w_in, w_out, y, hidden, act=ACT_SILU, residual=None, pre=None, transpose_w=False, stream=None):
+    """Gated feed-forward block (evkcu_gated_ffn): with [g | u] = x @ w_in,
+    hidden = act(g) * u and y = hidden @ w_out + residual.
+
+    x, y, residual (..., D); w_in (D, 2 F), w_out (F, D), or both transposed
+    with transpose_w; hidden (..., F); pre (..., 2 F) receives [g | u] for
+    gated_ffn_backward.  y = None (then w_out may be None) stops at hidden."""
+    D, F = x.shape[-1], hidden.shape[-1]
+    lead = tuple(x.shape[:-1])
+    _same("gated_ffn", x, dict(w_in=(w_in, (2 * F, D) if transpose_w else (D, 2 * F)),
+                               w_out=(w_out, (D, F) if transpose_w else (F, D)), y=(y, x.shape),
+                               hidden=(hidden, lead + (F,)), residual=(residual, x.shape),
+                               pre=(pre, lead + (2 * F,))))
+    _check("evkcu_gated_ffn", lib().evkcu_gated_ffn(
+        _ptr(x), _ptr(w_in), _ptr(w_out), _ptr(residual), _ptr(y), _ptr(hidden), _ptr(pre),
+        x.numel() // D if D else 0, D, F, act, MM_TRANSPOSE_B if transpose_w else 0, _dtype_code(x),
+        _stream(stream)))
+    return y if y is not None else hidden
+
+
+def gated_ffn_backward(x, w_in, w_out, pre, dy, dpre, hidden, dx=None, dw_in=None, dw_out=None, act=ACT_SILU,
+                       transpose_w=False, acc=False, stream=None):
+    """Gradients of gated_ffn from dy (evkcu_gated_ffn_backward) into those of
+    dx, dw_in and dw_out that are given; acc adds to them.  pre is gated_ffn's;
+    dpre (like pre; pre itself is allowed) receives its gradient; hidden
+    (..., F) is recomputed and needed only for dw_out."""
+    D, F = x.shape[-1], pre.shape[-1] // 2
+    lead = tuple(x.shape[:-1])
+    si, so = ((2 * F, D), (D, F)) if transpose_w else ((D, 2 * F), (F, D))
+    _same("gated_ffn_backward", x, dict(w_in=(w_in, si), w_out=(w_out, so), pre=(pre, lead + (2 * F,)),
+                                        dy=(dy, x.shape), dpre=(dpre, lead + (2 * F,)),
+                                        hidden=(hidden, lead + (F,)), dx=(dx, x.shape), dw_in=(dw_in, si),
+                                        dw_out=(dw_out, so)))
+    flags = (MM_TRANSPOSE_B if transpose_w else 0) | (MM_ACC_C if acc else 0)
+    _check("evkcu_gated_ffn_backward", lib().evkcu_gated_ffn_backward(
+        _ptr(x), _ptr(w_in), _ptr(w_out), _ptr(pre), _ptr(dy), _ptr(dpre), _ptr(hidden), _ptr(dx), _ptr(dw_in),
+        _ptr(dw_out), x.numel() // D if D else 0, D, F, act, flags, _dtype_code(x), _stream(stream)))
+    return dx, dw_in, dw_out
+
+
+def _rows(op, name, t, B, S, cols=None):
+    """(pointer, row pitch) of a (B, S, cols) tensor whose rows are evenly
+    spaced (a slice of the last dimension of a contiguous tensor is)."""
+    if not t.is_cuda:
+        raise ValueError("evk_b200 ops take CUDA tensors")
+    if t.dim() != 3 or t.shape[0] != B or t.shape[1] != S or (cols is not None and t.shape[2] != cols):
+        raise EvkcuError(op, 1, f"{name} is {tuple(t.shape)}, expected {(B, S, cols)}")
+    sb, st, sc = t.stride()
+    pitch = st if S > 1 else sb if B > 1 else max(t.shape[2], 1)
+    if (t.shape[2] > 1 and sc != 1) or (B > 1 and S > 1 and sb != S * st):
+        raise EvkcuError(op, 1, f"{name}: strides {t.stride()} are not evenly spaced rows")
+    return t.data_ptr(), pitch
+
+
+def _qk_desc(op, q, k, heads, q_out, k_out, positions, rot_dim, half_split, eps, base, pos_offset):
+    import torch
+
+    if q.dim() != 3 or heads <= 0 or q.shape[2] % heads:
+        raise EvkcuError(op, 1, f"q is {tuple(q.shape)}, expected (B, S, {heads} heads * head_dim)")
+    B, S = q.shape[:2]
+    dh = q.shape[2] // heads
+    kv = 0
+    if k is not None:
+        if dh == 0 or k.dim() != 3 or k.shape[2] % dh:
+            raise EvkcuError(op, 1, f"k is {tuple(k.shape)}, expected (B, S, kv_heads * {dh})")
+        kv = k.shape[2] // dh
+    pos = None
+    if positions is not None:
+        if positions.dtype != torch.int32 or positions.numel() != B * S or positions.device != q.device:
+            raise EvkcuError(op, 1, f"positions must be {B * S} int32 values on {q.device}")
+        pos = _ptr(positions)
+    if not 0 <= rot_dim <= 0xFFFFFFFF or not 0 <= pos_offset <= 0xFFFFFFFF:
+        raise EvkcuError(op, 1, "rot_dim and pos_offset must be non-negative")
+    d = QkNormRopeDesc(batch=B, seq_len=S, heads=heads, kv_heads=kv, head_dim=dh, rot_dim=rot_dim,
+                       flags=QK_HALF_SPLIT if half_split else 0, pos_offset=pos_offset, eps=eps, base=base,
+                       positions=pos)
+    return d, B, S, kv * dh
+
+
+def qk_norm_rope(q, k, q_out, k_out, heads: int, gain_q=None, gain_k=None, v=None, v_out=None, cache=False,
+                 positions=None, rot_dim=0, half_split=False, eps=1e-5, base=10000.0, pos_offset=0, stream=None):
+    """Per-head RMSNorm and rotation of queries and keys in one pass
+    (evkcu_qk_norm_rope).
+
+    q, q_out (B, S, heads * Dh); k, k_out (B, S, Hkv * Dh), or None for queries
+    only; rows may be slices of a fused QKV tensor.  gain_q, gain_k (Dh,).
+    positions: B * S int32 values, else pos_offset + t.  With cache=True, k_out
+    is a contiguous KV cache (B, cache_len, Hkv * Dh) and keys go to the rows of
+    their positions; v is copied along to v_out."""
+    op = "qk_norm_rope"
+    d, B, S, kc = _qk_desc(op, q, k, heads, q_out, k_out, positions, rot_dim, half_split, eps, base, pos_offset)
+    dh = d.head_dim
+    _same(op, q, dict(q_out=(q_out, q.shape), k=(k, (B, S, kc)), gain_q=(gain_q, (dh,)), gain_k=(gain_k, (dh,)),
+                      v=(v, (B, S, kc))))
+    qp, d.q_pitch = _rows(op, "q", q, B, S)
+    qo, d.q_out_pitch = _rows(op, "q_out", q_out, B, S)
+    kp = ko = vp = vo = None
+    if k is not None:
+        kp, d.k_pitch = _rows(op, "k", k, B, S)
+        if cache:
+            if k_out.dim() != 3:
+                raise EvkcuError(op, 1, f"k_out is {tuple(k_out.shape)}, expected (B, cache_len, {kc})")
+            d.flags |= QK_CACHE
+            d.cache_len = k_out.shape[1]
+            d.k_out_pitch = kc
+            _same(op, q, dict(k_out=(k_out, (B, d.cache_len, kc)), v_out=(v_out, k_out.shape)))
+            ko, vo = _ptr(k_out), _ptr(v_out)
+        else:
+            _same(op, q, dict(k_out=(k_out, (B, S, kc)), v_out=(v_out, (B, S, kc))))
+            ko, d.k_out_pitch = _rows(op, "k_out", k_out, B, S)
+            if v_out is not None:
+                vo, vpitch = _rows(op, "v_out", v_out, B, S)
+                if vpitch != d.k_out_pitch:
+                    raise EvkcuError(op, 1, "v_out must have the row pitch of k_out")
+        if v is not None:
+            vp, d.v_pitch = _rows(op, "v", v, B, S)
+    elif v is not None or v_out is not None or cache:
+        raise EvkcuError(op, 7, "v, v_out and cache need k")
+    _check("evkcu_qk_norm_rope", lib().evkcu_qk_norm_rope(
+        d, qp, kp, vp, _ptr(gain_q), _ptr(gain_k), qo, ko, vo, _dtype_code(q), _stream(stream)))
+    return q_out, k_out
+
+
+def qk_norm_rope_workspace(head_dim: int) -> int:
+    """Bytes of workspace that qk_norm_rope_backward needs for gain gradients."""
+    return int(lib().evkcu_qk_norm_rope_workspace(head_dim))
+
+
+def qk_norm_rope_backward(q, k, dq_out, dk_out, dq, dk, heads: int, gain_q=None, gain_k=None, dgain_q=None,
+                          dgain_k=None, workspace=None, positions=None, rot_dim=0, half_split=False, eps=1e-5,
+                          base=10000.0, pos_offset=0, acc_gain=False, stream=None):
+    """Gradients of qk_norm_rope (evkcu_qk_norm_rope_backward): from those of
+    its outputs and its saved inputs q, k into dq, dk (dq may be dq_out, dk may
+    be dk_out) and, where given, dgain_q, dgain_k (Dh,), which need a
+    `workspace` tensor of qk_norm_rope_workspace(Dh) bytes and are added to with
+    acc_gain."""
+    op = "qk_norm_rope_backward"
+    d, B, S, kc = _qk_desc(op, q, k, heads, dq_out, dk_out, positions, rot_dim, half_split, eps, base, pos_offset)
+    dh = d.head_dim
+    _same(op, q, dict(dq_out=(dq_out, q.shape), dq=(dq, q.shape), gain_q=(gain_q, (dh,)), gain_k=(gain_k, (dh,)),
+                      dgain_q=(dgain_q, (dh,)), dgain_k=(dgain_k, (dh,))))
+    if acc_gain:
+        d.flags |= QK_ACC_GAIN
+    qp, d.q_pitch = _rows(op, "q", q, B, S)
+    gq, d.q_out_pitch = _rows(op, "dq_out", dq_out, B, S)
+    dqp, d.dq_pitch = _rows(op, "dq", dq, B, S)
+    kp = gk = dkp = None
+    if k is not None:
+        _same(op, q, dict(k=(k, (B, S, kc)), dk_out=(dk_out, k.shape), dk=(dk, k.shape)))
+        kp, d.k_pitch = _rows(op, "k", k, B, S)
+        gk, d.k_out_pitch = _rows(op, "dk_out", dk_out, B, S)
+        dkp, d.dk_pitch = _rows(op, "dk", dk, B, S)
+    wbytes = 0
+    if workspace is not None:
+        if workspace.device != q.device:
+            raise EvkcuError(op, 7, f"workspace is on {workspace.device}, expected {q.device}")
+        wbytes = workspace.numel() * workspace.element_size()
+    _check("evkcu_qk_norm_rope_backward", lib().evkcu_qk_norm_rope_backward(
+        d, qp, kp, _ptr(gain_q), _ptr(gain_k), gq, gk, dqp, dkp, _ptr(dgain_q), _ptr(dgain_k), _ptr(workspace), wbytes,
+        _dtype_code(q), _stream(stream)))
+    return dq, dk
 
 
 # ------------------------------------------------------------- LLM driver --

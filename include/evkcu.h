@@ -54,6 +54,20 @@ typedef enum evkcu_dtype {
  * sum_j p_ij dp_ij (= t_i / l_i) instead of the reference shader's t_i.     */
 #define EVKCU_ATTN_BWD_NORMALIZED 2u
 
+/* activations of evkcu_linear / evkcu_gated_ffn (extension); GELU is the tanh
+ * form of evkcu_gelu                                                         */
+typedef enum evkcu_act {
+    EVKCU_ACT_NONE = 0,
+    EVKCU_ACT_RELU = 1,
+    EVKCU_ACT_GELU = 2,
+    EVKCU_ACT_SILU = 3
+} evkcu_act;
+
+/* evkcu_qk_norm_rope flags */
+#define EVKCU_QK_HALF_SPLIT 1u /* pairs (i, i + rot_dim / 2) instead of (2 i, 2 i + 1) */
+#define EVKCU_QK_CACHE 2u      /* keys and values go to their rows of a KV cache       */
+#define EVKCU_QK_ACC_GAIN 4u   /* backward: dgain += instead of =                      */
+
 /* ---- context -------------------------------------------------------------
  * Replaces evk::ai::initialize / shutdown (evk_ai.h:489-490, evk_ai.cpp:211-252):
  * selects the device and creates the per-device state (SM count, device error
@@ -280,6 +294,105 @@ int evkcu_cross_entropy_loss(const void* logits, const void* targets, void* grad
 int evkcu_flash_attention_bwd(const void* q, const void* k, const void* v, const void* o, const void* dO, void* dQ,
                               void* dK, void* dV, uint32_t B, uint32_t N, uint32_t H, uint32_t Hkv, uint32_t Dh,
                               float scale, uint32_t flags, int dtype, void* stream);
+
+/* ---- decoder-layer operators around attention (extension) ------------------
+ * No counterparts in the reference, whose layers compose matmul, gelu, add,
+ * rms_norm and rope (example/main_llm.cpp:528-546).  Shared rules:
+ *   - matrices are contiguous, 16-byte aligned; K, N, D and F are positive
+ *     multiples of 8; any number of rows, 0 included (then the gradients of
+ *     the weights and the bias are 0);
+ *   - products accumulate in fp32 and every output is rounded once.  Tensors
+ *     that the call itself reads back (dpre, hidden) are rounded to the
+ *     storage type in between, as tensor-core operands have to be;
+ *   - nothing is allocated and no scratch is shared between calls: what a call
+ *     needs besides its outputs it gets as an argument, so calls on several
+ *     streams and captured graphs are independent as long as their buffers are;
+ *   - an output that shares memory with another argument is refused
+ *     (EVKCU_BAD_ARG) but for the cases named below;
+ *   - results do not depend on timing: equal calls give equal bits.          */
+
+/* z = x W + bias;  pre = z;  y = act(z) + residual.
+ * x [rows, K];  W [K, N], or [N, K] with EVKCU_MM_TRANSPOSE_B (the only flag);
+ * bias [N], residual [rows, N] (y itself is allowed) and pre [rows, N]
+ * (receives z, for the backward pass) may be NULL.  The activation applies to
+ * the unrounded z.                                                           */
+int evkcu_linear(const void* x, const void* w, const void* bias, const void* residual, void* y, void* pre,
+                 uint32_t rows, uint32_t K, uint32_t N, int act, uint32_t flags, int dtype, void* stream);
+
+/* Gradients of evkcu_linear from dy [rows, N] and the saved pre:
+ * dz = dy act'(pre);  dx = dz W^T;  dW = x^T dz (stored as W is);
+ * dbias = column sums of dz (unrounded).  dx, dw and dbias may each be NULL
+ * (not computed); with EVKCU_MM_ACC_C they are added to what is there.
+ * With an activation, dpre [rows, N] receives dz (it may be pre or dy
+ * itself); without one, pre and dpre are not used.  The residual's gradient is
+ * dy.  The derivative of RELU at 0 is 0.                                     */
+int evkcu_linear_backward(const void* x, const void* w, const void* pre, const void* dy, void* dpre, void* dx,
+                          void* dw, void* dbias, uint32_t rows, uint32_t K, uint32_t N, int act, uint32_t flags,
+                          int dtype, void* stream);
+
+/* Gated feed-forward block:
+ * [g | u] = x W_in;  pre = [g | u];  hidden = act(g) u;  y = hidden W_out + residual.
+ * x, y [rows, D]; W_in [D, 2 F] (gate columns, then up columns); W_out [F, D];
+ * with EVKCU_MM_TRANSPOSE_B both weights are stored transposed ([2 F, D] and
+ * [D, F]).  hidden [rows, F] is an output and the second product's operand;
+ * pre [rows, 2 F] (for the backward pass) and residual [rows, D] (y itself is
+ * allowed) may be NULL; y = NULL stops at hidden (a gated linear unit).      */
+int evkcu_gated_ffn(const void* x, const void* w_in, const void* w_out, const void* residual, void* y, void* hidden,
+                    void* pre, uint32_t rows, uint32_t D, uint32_t F, int act, uint32_t flags, int dtype,
+                    void* stream);
+
+/* Gradients of evkcu_gated_ffn from dy [rows, D] and the saved pre:
+ * dh = dy W_out^T (fp32, never stored);  dpre = [dh u act'(g) | dh act(g)];
+ * dx = dpre W_in^T;  dW_in = x^T dpre;  dW_out = hidden^T dy.
+ * dpre [rows, 2 F] is an output (pre itself is allowed); hidden [rows, F]
+ * receives act(g) u again (the forward pass's need not be kept) and is used
+ * only with dw_out.  dx, dw_in, dw_out may each be NULL; with EVKCU_MM_ACC_C
+ * they are added to what is there.  The residual's gradient is dy.           */
+int evkcu_gated_ffn_backward(const void* x, const void* w_in, const void* w_out, const void* pre, const void* dy,
+                             void* dpre, void* hidden, void* dx, void* dw_in, void* dw_out, uint32_t rows, uint32_t D,
+                             uint32_t F, int act, uint32_t flags, int dtype, void* stream);
+
+/* Shapes of evkcu_qk_norm_rope.  Rows are (sequence b, token t), b-major; a
+ * tensor's row r starts r * pitch elements after its first (pitches are
+ * multiples of 8), so slices of a fused QKV projection are taken as they lie.
+ * The position of a row is positions[r], or pos_offset + t without positions. */
+typedef struct evkcu_qk_norm_rope_desc {
+    uint32_t batch, seq_len, heads, kv_heads; /* kv_heads = 0: queries only           */
+    uint32_t head_dim;                        /* a multiple of 8, 8 to 256            */
+    uint32_t rot_dim;                         /* rotated part of a head; 0: all of it */
+    uint32_t flags, pos_offset;
+    uint32_t cache_len; /* EVKCU_QK_CACHE: rows of each sequence's cache              */
+    float eps, base;
+    const int32_t* positions; /* [batch * seq_len] in device memory, or NULL           */
+    uint64_t q_pitch, k_pitch, v_pitch, q_out_pitch, k_out_pitch, dq_pitch, dk_pitch;
+} evkcu_qk_norm_rope_desc;
+
+/* Every query and key head x of head_dim values: x rsqrt(mean(x^2) + eps) *
+ * gain, then the rotation of its first rot_dim values by position *
+ * base^(-2 i / rot_dim), in one pass with one rounding; the angles are reduced
+ * in 64 bits, so far positions are exact.  gain_q, gain_k [head_dim] or NULL.
+ * q_out may be q, k_out k and v_out v (same pitch; not into a cache).
+ * With EVKCU_QK_CACHE, k_out is a cache [batch, cache_len, kv_heads *
+ * head_dim] (rows k_out_pitch apart) and each key goes to the row of its
+ * position; rows at positions outside [0, cache_len) are not stored, and
+ * positions of one sequence have to differ.  v (optional) is copied unchanged
+ * to v_out, which is laid out as k_out.                                      */
+int evkcu_qk_norm_rope(const evkcu_qk_norm_rope_desc* d, const void* q, const void* k, const void* v,
+                       const void* gain_q, const void* gain_k, void* q_out, void* k_out, void* v_out, int dtype,
+                       void* stream);
+
+/* Gradients from those of the outputs (dq_out, dk_out; rows q_out_pitch and
+ * k_out_pitch apart) and the saved inputs q, k: dq, dk are overwritten (dq may
+ * be dq_out, dk may be dk_out, with the same pitch), dgain_q / dgain_k
+ * [head_dim] are summed over rows and heads (each may be NULL; added to with
+ * EVKCU_QK_ACC_GAIN).  The gain gradients need a workspace of
+ * evkcu_qk_norm_rope_workspace(head_dim) bytes that no other call uses at the
+ * same time; its contents do not matter.                                     */
+int evkcu_qk_norm_rope_backward(const evkcu_qk_norm_rope_desc* d, const void* q, const void* k, const void* gain_q,
+                                const void* gain_k, const void* dq_out, const void* dk_out, void* dq, void* dk,
+                                void* dgain_q, void* dgain_k, void* workspace, uint64_t workspace_bytes, int dtype,
+                                void* stream);
+uint64_t evkcu_qk_norm_rope_workspace(uint32_t head_dim);
 
 /* ---- LLM driver (extension) ------------------------------------------------
  * The decoder that example/main_llm.cpp builds from these operators
