@@ -408,9 +408,9 @@ int launch_decode(const void* q, const void* k, const void* v, void* o, uint32_t
     CUtensorMap mK, mV;
     const uint64_t pitch = (uint64_t)Hkv * Dh, rows = (uint64_t)B * max_len;
     const int dt = std::is_same<T, __nv_bfloat16>::value ? EVKCU_BF16 : EVKCU_F16;
-    int r = make_tmap_3d(&mK, k, pitch, rows, 1, pitch, pitch * rows, Dh, ROWS, dt, false);
+    int r = make_tmap_3d(&mK, k, pitch, rows, 1, pitch, pitch * rows, Dh, ROWS, dt, 0);
     if (r) return r;
-    r = make_tmap_3d(&mV, v, pitch, rows, 1, pitch, pitch * rows, Dh, ROWS, dt, false);
+    r = make_tmap_3d(&mV, v, pitch, rows, 1, pitch, pitch * rows, Dh, ROWS, dt, 0);
     if (r) return r;
     dim3 grid(nsplit, Hkv * hgroups, B);
     return launch_pdl("evkcu_single_query_attention", kern, grid, kDecThreads, smem, st, mK, mV, (const T*)q, (T*)o, H,

@@ -11,9 +11,12 @@
 // Every product runs on tcgen05 with fp32 accumulators and an epilogue of
 // linear.cuh.  Transposed operands are MN-major descriptors, never copies.
 #include <algorithm>
+#include <atomic>
+#include <cstring>
 #include <string>
 
 #include "linear.cuh"
+#include "linear_pair.cuh"
 #include "sm100.cuh"
 
 namespace evkcu {
@@ -197,18 +200,33 @@ struct Product {
     cudaStream_t st;
 };
 
+// Sets a kernel's shared-memory limit once per device.
+template <class K>
+int allow_smem(K* kern, int bytes, std::atomic<uint64_t>& done) {
+    const uint64_t bit = 1ull << (state()->device & 63);
+    if (done.load(std::memory_order_relaxed) & bit) return EVKCU_OK;
+    EVKCU_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return EVKCU_OK;
+}
+
+// Operand maps; box_b: rows of a box of B stored [nb, K].
+template <bool A_MN, bool B_MN>
+int operand_maps(const Product& p, CUtensorMap* ta, CUtensorMap* tb, uint32_t box_b) {
+    EVKCU_TRY(A_MN ? make_tmap_3d(ta, p.A, p.M, p.K, 1, p.M, (uint64_t)p.M * p.K, 64, BK, p.dtype)
+                   : make_tmap_3d(ta, p.A, p.K, p.M, 1, p.K, (uint64_t)p.M * p.K, BK, BM, p.dtype));
+    return B_MN ? make_tmap_3d(tb, p.B, p.nb, p.K, 1, p.nb, (uint64_t)p.nb * p.K, 64, BK, p.dtype)
+                : make_tmap_3d(tb, p.B, p.K, p.nb, 1, p.K, (uint64_t)p.nb * p.K, BK, box_b, p.dtype);
+}
+
 template <typename T, int BN, bool A_MN, bool B_MN, class Epi>
 int launch_tile(const Product& p, const Epi& epi) {
     using Cfg = TileCfg<BN>;
     CUtensorMap ta, tb;
-    int r = A_MN ? make_tmap_3d(&ta, p.A, p.M, p.K, 1, p.M, (uint64_t)p.M * p.K, 64, BK, p.dtype)
-                 : make_tmap_3d(&ta, p.A, p.K, p.M, 1, p.K, (uint64_t)p.M * p.K, BK, BM, p.dtype);
-    if (!r)
-        r = B_MN ? make_tmap_3d(&tb, p.B, p.nb, p.K, 1, p.nb, (uint64_t)p.nb * p.K, 64, BK, p.dtype)
-                 : make_tmap_3d(&tb, p.B, p.K, p.nb, 1, p.K, (uint64_t)p.nb * p.K, BK, 64, p.dtype);
-    if (r) return r;
+    EVKCU_TRY((operand_maps<A_MN, B_MN>(p, &ta, &tb, 64)));
     auto kern = tile_kernel<T, BN, A_MN, B_MN, Epi>;
-    EVKCU_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
+    static std::atomic<uint64_t> done{0};
+    EVKCU_TRY(allow_smem(kern, Cfg::SMEM, done));
     constexpr uint32_t COLS = Epi::kGated ? BN / 2 : BN;
     const dim3 grid((p.N + COLS - 1) / COLS, (p.M + BM - 1) / BM);
     const uint32_t idesc = make_idesc_f16(BM, BN, p.dtype == EVKCU_BF16 ? 1 : 0, A_MN, B_MN);
@@ -216,13 +234,87 @@ int launch_tile(const Product& p, const Epi& epi) {
     return after_launch("evkcu_linear(tile)");
 }
 
+// The staged form of each epilogue: its boxes' maps (128 rows x 32 columns of
+// a [M, N] matrix with rows of `pitch` elements) and parameters.
+int box_map(CUtensorMap* m, const void* p, const Product& pr, uint64_t pitch) {
+    return make_tmap_3d(m, p, pr.N, pr.M, 1, pitch, pitch * pr.M, 32, 128, pr.dtype, 64);
+}
+template <typename T>
+int stage(const Product& p, const EpiLinear<T>& e, pairk::Maps& m, pairk::StagedLinear<T>& s) {
+    s = pairk::StagedLinear<T>{e.bias, e.N, e.act, e.res != nullptr, e.pre != nullptr};
+    if (e.res) EVKCU_TRY(box_map(&m.in0, e.res, p, p.N));
+    if (e.pre) EVKCU_TRY(box_map(&m.out1, e.pre, p, p.N));
+    return box_map(&m.out0, e.y, p, p.N);
+}
+template <typename T>
+int stage(const Product& p, const EpiGated<T>& e, pairk::Maps& m, pairk::StagedGated<T>& s) {
+    s = pairk::StagedGated<T>{e.act, e.pre != nullptr};
+    if (e.pre) {
+        EVKCU_TRY(box_map(&m.out1, e.pre, p, 2 * (uint64_t)p.N));
+        EVKCU_TRY(box_map(&m.out2, e.pre + p.N, p, 2 * (uint64_t)p.N));
+    }
+    return box_map(&m.out0, e.h, p, p.N);
+}
+template <typename T>
+int stage(const Product& p, const EpiGatedBwd<T>& e, pairk::Maps& m, pairk::StagedGatedBwd<T>& s) {
+    s = pairk::StagedGatedBwd<T>{e.act, e.h != nullptr};
+    const uint64_t pitch = 2 * (uint64_t)p.N;
+    EVKCU_TRY(box_map(&m.in0, e.pre, p, pitch));
+    EVKCU_TRY(box_map(&m.in1, e.pre + p.N, p, pitch));
+    EVKCU_TRY(box_map(&m.out0, e.dpre, p, pitch));
+    EVKCU_TRY(box_map(&m.out1, e.dpre + p.N, p, pitch));
+    return e.h ? box_map(&m.out2, e.h, p, p.N) : (int)EVKCU_OK;
+}
+template <class Epi> struct StagedOf;
+template <typename T> struct StagedOf<EpiLinear<T>> { using type = pairk::StagedLinear<T>; };
+template <typename T> struct StagedOf<EpiGated<T>> { using type = pairk::StagedGated<T>; };
+template <typename T> struct StagedOf<EpiGatedBwd<T>> { using type = pairk::StagedGatedBwd<T>; };
+
+template <typename T, bool A_MN, bool B_MN, class Epi>
+int launch_pair(const Product& p, const Epi& epi) {
+    using S = typename StagedOf<Epi>::type;
+    DeviceState* ds = state();
+    auto kern = pairk::pair_kernel<T, A_MN, B_MN, S>;
+    static std::atomic<uint64_t> done{0};
+    EVKCU_TRY(allow_smem(kern, pairk::SMEM, done));
+    if (!ds->linear_clusters) {  // equal for every instantiation: one CTA per SM
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(2 * (ds->sm_count / 2));
+        cfg.blockDim = dim3(pairk::THREADS);
+        cfg.dynamicSmemBytes = pairk::SMEM;
+        int n = 0;
+        EVKCU_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
+        ds->linear_clusters = std::max(n, 1);
+    }
+    pairk::Maps maps;
+    memset(&maps, 0, sizeof(maps));
+    S s;
+    EVKCU_TRY((operand_maps<A_MN, B_MN>(p, &maps.a, &maps.b, 128)));
+    EVKCU_TRY(stage(p, epi, maps, s));
+    constexpr uint64_t COLS = Epi::kGated ? 128 : 256;
+    const uint64_t tiles = ((uint64_t)p.M + 255) / 256 * ((p.N + COLS - 1) / COLS);
+    EVKCU_CHECK_ARG(tiles <= 0xFFFFFFFFu / 2, EVKCU_BAD_SHAPE, "evkcu_linear: too many output tiles");
+    const uint32_t grid = 2 * (uint32_t)std::min<uint64_t>(tiles, (uint64_t)ds->linear_clusters);
+    const uint32_t idesc = make_idesc_f16(256, 256, p.dtype == EVKCU_BF16 ? 1 : 0, A_MN, B_MN);
+    kern<<<grid, pairk::THREADS, pairk::SMEM, p.st>>>(maps, s, p.M, p.N, p.K, idesc, ds->d_error);
+    return after_launch("evkcu_linear(pair)");
+}
+
+template <typename T, bool A_MN, bool B_MN, class Epi>
+int launch_product(const Product& p, const Epi& epi) {
+    constexpr uint64_t COLS = Epi::kGated ? 128 : 256;
+    const uint64_t pair_tiles = ((uint64_t)p.M + 255) / 256 * ((p.N + COLS - 1) / COLS);
+    if (pair_tiles >= 40) return launch_pair<T, A_MN, B_MN>(p, epi);
+    return launch_tile<T, 128, A_MN, B_MN>(p, epi);
+}
+
 // A transposed A (weight gradients) always comes with a B stored [K, nb].
 template <typename T, bool A_MN, class Epi>
 int product(const Product& p, const Epi& epi) {
     if constexpr (!A_MN) {
-        if (!p.b_mn) return launch_tile<T, 128, false, false>(p, epi);
+        if (!p.b_mn) return launch_product<T, false, false>(p, epi);
     }
-    return launch_tile<T, 128, A_MN, true>(p, epi);
+    return launch_product<T, A_MN, true>(p, epi);
 }
 
 // -------------------------------- dz = dy act'(z) and its column sums ----

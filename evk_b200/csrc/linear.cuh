@@ -107,6 +107,42 @@ __device__ __forceinline__ void act_both(float z, int act, float& a, float& da) 
     }
 }
 
+// Eight values at once, the activation chosen outside the loop.
+__device__ __forceinline__ void act8(float (&f)[8], int act) {
+    if (act == EVKCU_ACT_NONE) return;
+    if (act == EVKCU_ACT_SILU) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = act_f(f[e], EVKCU_ACT_SILU);
+    } else if (act == EVKCU_ACT_GELU) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = act_f(f[e], EVKCU_ACT_GELU);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = act_f(f[e], EVKCU_ACT_RELU);
+    }
+}
+
+// dg = dh u act'(g), du = dh act(g), h = act(g) u
+template <int ACT>
+__device__ __forceinline__ void gated_bwd8_of(const float (&dh)[8], const float (&g)[8], const float (&u)[8],
+                                              float (&dg)[8], float (&du)[8], float (&h)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        float a, da;
+        act_both(g[e], ACT, a, da);
+        dg[e] = dh[e] * u[e] * da;
+        du[e] = dh[e] * a;
+        h[e] = a * u[e];
+    }
+}
+__device__ __forceinline__ void gated_bwd8(const float (&dh)[8], const float (&g)[8], const float (&u)[8],
+                                           float (&dg)[8], float (&du)[8], float (&h)[8], int act) {
+    if (act == EVKCU_ACT_SILU) gated_bwd8_of<EVKCU_ACT_SILU>(dh, g, u, dg, du, h);
+    else if (act == EVKCU_ACT_GELU) gated_bwd8_of<EVKCU_ACT_GELU>(dh, g, u, dg, du, h);
+    else if (act == EVKCU_ACT_RELU) gated_bwd8_of<EVKCU_ACT_RELU>(dh, g, u, dg, du, h);
+    else gated_bwd8_of<EVKCU_ACT_NONE>(dh, g, u, dg, du, h);
+}
+
 __device__ __forceinline__ Vec8 ld_vec8(const void* p) { return *reinterpret_cast<const Vec8*>(p); }
 __device__ __forceinline__ void st_vec8(void* p, const Vec8& v) { *reinterpret_cast<Vec8*>(p) = v; }
 
@@ -135,10 +171,7 @@ struct EpiLinear {
             for (int e = 0; e < 8; ++e) f[e] += t[e];
         }
         if (pre) st_vec8(pre + at, pack8<T>(f));
-        if (act != EVKCU_ACT_NONE) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = act_f(f[e], act);
-        }
+        act8(f, act);
         if (res) {
             unpack8<T>(ld_vec8(res + at), t);
 #pragma unroll
@@ -162,10 +195,10 @@ struct EpiGated {
             st_vec8(p, pack8<T>(g));
             st_vec8(p + F, pack8<T>(u));
         }
-        float f[8];
+        act8(g, act);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = act_f(g[e], act) * u[e];
-        st_vec8(h + (uint64_t)row * F + col, pack8<T>(f));
+        for (int e = 0; e < 8; ++e) g[e] *= u[e];
+        st_vec8(h + (uint64_t)row * F + col, pack8<T>(g));
     }
 };
 
@@ -184,14 +217,7 @@ struct EpiGatedBwd {
         float g[8], u[8], dg[8], du[8], hh[8];
         unpack8<T>(ld_vec8(pre + at), g);
         unpack8<T>(ld_vec8(pre + at + F), u);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            float a, da;
-            act_both(g[e], act, a, da);
-            dg[e] = dh[e] * u[e] * da;
-            du[e] = dh[e] * a;
-            hh[e] = a * u[e];
-        }
+        gated_bwd8(dh, g, u, dg, du, hh, act);
         st_vec8(dpre + at, pack8<T>(dg));
         st_vec8(dpre + at + F, pack8<T>(du));
         if (h) st_vec8(h + (uint64_t)row * F + col, pack8<T>(hh));

@@ -424,10 +424,10 @@ __device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
 }  // namespace sm100
 
 // Host: encodes a 3-D tiled tensor map through the driver entry point (no
-// link-time dependency on libcuda), 128-byte swizzled by default, else a
-// dense row-major box.  dims/strides in elements of 2 bytes; box in elements.
+// link-time dependency on libcuda), 128-byte swizzled by default, else 64-byte
+// swizzled (64) or a dense row-major box (0).  dims/strides in elements of 2 bytes; box in elements.
 // Returns EVKCU_OK or an error status.
 int make_tmap_3d(CUtensorMap* map, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t stride1_elems,
-                 uint64_t stride2_elems, uint32_t box0, uint32_t box1, int dtype, bool swizzle128 = true);
+                 uint64_t stride2_elems, uint32_t box0, uint32_t box1, int dtype, uint32_t swizzle = 128);
 
 }  // namespace evkcu

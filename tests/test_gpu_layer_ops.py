@@ -115,6 +115,13 @@ KN = [(8, 8), (64, 56), (72, 136), (264, 72), (520, 264), (1024, 520)]
 LINEAR = [(r, *KN[(i + j) % len(KN)], list(ACTS)[(i + j) % 4], DTYPES[(i // 2 + j) % 2], bool((i + j) % 2),
            bool(i % 3), bool((i + j) % 3 == 1), bool((i // 3 + j) % 2)) for i, r in enumerate(ROWS) for j in range(4)]
 
+# Outputs of many tiles: several rounds of a persistent grid, ragged at every edge.
+LINEAR += [(4100, 72, 4104, "gelu", torch.bfloat16, True, True, True, False),
+           (4100, 200, 4104, "none", torch.float16, True, False, False, True),
+           (2305, 1024, 1800, "silu", torch.float16, False, True, False, False),
+           (129, 264, 16392, "relu", torch.bfloat16, False, False, True, True),
+           (16385, 64, 264, "none", torch.bfloat16, False, True, False, False)]
+
 
 @pytest.mark.parametrize("rows,K,N,act,dt,bias,res,pre,nk", LINEAR)
 def test_linear(rows, K, N, act, dt, bias, res, pre, nk):
@@ -165,6 +172,9 @@ def back_ref(x, w, z, dy, act, dt):
 
 BACK = [(r, *KN[(i + 2 * j) % len(KN)], list(ACTS)[(i + j) % 4], DTYPES[(i // 2 + j) % 2], bool((i // 2 + j) % 2),
          bool(i % 2 == j)) for i, r in enumerate([1, 7, 64, 100, 129, 257, 1000]) for j in range(2)]
+
+BACK += [(1001, 2056, 1800, "gelu", torch.bfloat16, False, False), (300, 4104, 2056, "silu", torch.float16, True, True),
+         (5000, 264, 520, "relu", torch.float16, False, True), (2305, 1800, 2056, "none", torch.bfloat16, True, False)]
 
 
 @pytest.mark.parametrize("rows,K,N,act,dt,nk,acc", BACK)
@@ -232,6 +242,9 @@ DF = [(8, 8), (64, 72), (72, 200), (264, 136), (512, 1368)]
 FFN = [(r, *DF[(i + j) % len(DF)], list(ACTS)[(i + 2 * j) % 4], DTYPES[(i + j) % 2], bool(i % 2), bool((i + j) % 3),
         bool((i // 2 + j) % 2)) for i, r in enumerate(ROWS) for j in range(3)]
 
+FFN += [(2100, 520, 1368, "silu", torch.bfloat16, True, True, False), (1001, 72, 2056, "gelu", torch.float16, True, True, True),
+        (4097, 264, 1032, "relu", torch.bfloat16, False, False, True), (300, 2056, 4104, "silu", torch.float16, True, False, False)]
+
 
 @pytest.mark.parametrize("rows,D,F,act,dt,res,pre,nk", FFN)
 def test_gated_ffn(rows, D, F, act, dt, res, pre, nk):
@@ -274,6 +287,9 @@ def ffn_back_ref(x, wi, wo, z, dy, act, dt):
 
 FFNB = [(r, *DF[(i + j) % len(DF)], list(ACTS)[(i + 2 * j) % 4], DTYPES[(i + j) % 2], bool((i // 2 + j) % 2),
          bool(i % 2 == j)) for i, r in enumerate([1, 7, 64, 100, 129, 257, 1000]) for j in range(2)]
+
+FFNB += [(2100, 520, 1368, "silu", torch.bfloat16, False, False), (1001, 72, 2056, "gelu", torch.float16, True, True),
+         (4097, 264, 1032, "relu", torch.bfloat16, True, False), (300, 2056, 4104, "silu", torch.float16, False, True)]
 
 
 @pytest.mark.parametrize("rows,D,F,act,dt,nk,acc", FFNB)
