@@ -9,195 +9,38 @@
 //     dx = dpre [Wg | Wu]^T;  d[Wg | Wu] = x^T dpre;  dWd = h^T dy
 //
 // Every product runs on tcgen05 with fp32 accumulators and an epilogue of
-// linear.cuh.  Transposed operands are MN-major descriptors, never copies.
+// linear.cuh, in the paired-SM kernel (linear_pair.cuh) or the slab kernel
+// (linear_slab.cuh).  Transposed operands are MN-major descriptors, never
+// copies.
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstring>
 #include <string>
 
 #include "linear.cuh"
 #include "linear_pair.cuh"
+#include "linear_slab.cuh"
 #include "sm100.cuh"
 
 namespace evkcu {
 namespace {
 
-using namespace sm100;
-
-constexpr int BM = 128;
-constexpr int BK = 64;
-constexpr uint32_t kTimeoutTile = 0x601;
-
-// ------------------------------------------------- 128 x BN tile kernel ----
-// One CTA per 128 x BN output tile.  Warp 0 feeds 64-deep k-blocks by TMA
-// into a ring, warp 1 issues tcgen05.mma into a 128 x BN accumulator; warps
-// 2-5 then copy the accumulator to the (now idle) ring as fp32 and all warps
-// run the epilogue on eight consecutive columns at a time, so every global
-// access of the epilogue is a 16-byte one next to its neighbour lane's.
-// B arrives in boxes of 64 of its rows (or columns): a gated tile takes its
-// first box from the gate half of the weight and its second from the up
-// half, so accumulator columns c and c + 64 belong to the same hidden unit.
-template <int BN>
-struct TileCfg {
-    static constexpr int A_BYTES = BM * BK * 2;
-    static constexpr int B_BYTES = BN * BK * 2;
-    static constexpr int STAGE = A_BYTES + B_BYTES;
-    static constexpr int STAGES = 6;
-    static constexpr int LD = BN + 4;  // floats per staged row (16-byte rows on different banks)
-    static constexpr int SMEM = STAGES * STAGE + 1024 /*align*/ + 256 /*barriers*/;
-    static_assert(STAGES * STAGE >= BM * LD * 4, "the staged accumulator must fit in the ring");
-};
-constexpr int kTileThreads = 192;
-
-template <typename T, int BN, bool A_MN, bool B_MN, class Epi>
-__global__ void __launch_bounds__(kTileThreads, 1)
-    tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, Epi epi, uint32_t M,
-                uint32_t N, uint32_t K, uint32_t up_off, uint32_t idesc, unsigned int* err) {
-    using Cfg = TileCfg<BN>;
-    constexpr int STAGES = Cfg::STAGES;
-    constexpr uint32_t COLS = Epi::kGated ? BN / 2 : BN;  // output columns of a tile
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* sA = smem;
-    uint8_t* sB = smem + STAGES * Cfg::A_BYTES;
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * Cfg::STAGE);
-    uint64_t* empty = full + STAGES;
-    uint64_t* accum = empty + STAGES;
-    uint32_t* s_tmem = reinterpret_cast<uint32_t*>(accum + 1);
-    volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
-
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t n0 = blockIdx.x * COLS, m0 = blockIdx.y * BM;
-    const uint32_t num_kb = (K + BK - 1) / BK;
-
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) {
-            mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 1);
-        }
-        mbar_init(accum, 1);
-        *s_abort = 0;
-        fence_barrier_init();
-        prefetch_tmap(&tmA);
-        prefetch_tmap(&tmB);
-    }
-    if (warp == 1) {
-        tmem_alloc(s_tmem, BN);
-        tmem_relinquish();
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = *s_tmem;
-
-    uint32_t issued = 0;  // k-blocks requested (thread 0)
-    if (warp == 0) {
-        if (lane == 0) {
-            for (uint32_t kb = 0; kb < num_kb; ++kb) {
-                const int s = (int)(kb % STAGES);
-                if (!mbar_wait(&empty[s], ((kb / STAGES) & 1) ^ 1, s_abort, err, kTimeoutTile)) break;
-                mbar_arrive_expect_tx(&full[s], Cfg::STAGE);
-                const int k0 = (int)(kb * BK);
-                uint8_t* a = sA + s * Cfg::A_BYTES;
-                uint8_t* b = sB + s * Cfg::B_BYTES;
-                if (!A_MN) {
-                    tma_load_3d(a, &tmA, &full[s], k0, (int)m0, 0);
-                } else {
-                    tma_load_3d(a, &tmA, &full[s], (int)m0, k0, 0);
-                    tma_load_3d(a + 8192, &tmA, &full[s], (int)m0 + 64, k0, 0);
-                }
-#pragma unroll
-                for (int j = 0; j < BN / 64; ++j) {
-                    const int nb = Epi::kGated ? (int)(n0 + (uint32_t)j * up_off) : (int)n0 + 64 * j;
-                    if (!B_MN) tma_load_3d(b + j * 8192, &tmB, &full[s], k0, nb, 0);
-                    else tma_load_3d(b + j * 8192, &tmB, &full[s], nb, k0, 0);
-                }
-                issued = kb + 1;
-            }
-        }
-    } else if (warp == 1) {
-        if (lane == 0) {
-            bool ok = true;
-            for (uint32_t kb = 0; kb < num_kb; ++kb) {
-                const int s = (int)(kb % STAGES);
-                if (!mbar_wait(&full[s], (kb / STAGES) & 1, s_abort, err, kTimeoutTile)) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
-                const uint32_t a = smem_u32(sA + s * Cfg::A_BYTES);
-                const uint32_t b = smem_u32(sB + s * Cfg::B_BYTES);
-#pragma unroll
-                for (int k = 0; k < BK / 16; ++k) {
-                    const uint64_t ad =
-                        A_MN ? make_sw128_desc(a + k * 2048, 8192, 1024) : make_sw128_desc(a + k * 32, 16, 1024);
-                    const uint64_t bd =
-                        B_MN ? make_sw128_desc(b + k * 2048, 8192, 1024) : make_sw128_desc(b + k * 32, 16, 1024);
-                    mma_f16_ss(tmem, ad, bd, idesc, (kb | k) != 0);
-                }
-                mma_commit(&empty[s]);
-            }
-            if (ok) mma_commit(accum);
-        }
-    }
-    float* stage = reinterpret_cast<float*>(smem);
-    if (warp >= 2) {
-        const int q = warp & 3;  // TMEM lane quarter of this warp
-        const bool ok = __shfl_sync(0xffffffffu,
-                                    lane == 0 ? (int)mbar_wait_sleep(accum, 0, s_abort, err, kTimeoutTile) : 0,
-                                    0) != 0;
-        tc_fence_after();
-        if (ok) {
-            float* row = stage + (q * 32 + lane) * Cfg::LD;
-#pragma unroll 1
-            for (int c = 0; c < BN / 32; ++c) {
-                uint32_t r[32];
-                tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + c * 32, r);
-                tmem_wait_ld();
-#pragma unroll
-                for (int g = 0; g < 8; ++g)
-                    *reinterpret_cast<uint4*>(row + c * 32 + g * 4) =
-                        make_uint4(r[4 * g], r[4 * g + 1], r[4 * g + 2], r[4 * g + 3]);
-            }
-        }
-        tc_fence_before();
-    }
-    __syncthreads();
-    if (warp == 1) {
-        tc_fence_after();
-        tmem_dealloc(tmem, BN);
-    }
-    if (*s_abort) {
-        // A wait gave up: the copies in flight land before the CTA leaves.
-        if (threadIdx.x == 0)
-            for (uint32_t i = issued > STAGES ? issued - STAGES : 0; i < issued; ++i)
-                mbar_drain(&full[i % STAGES], (i / STAGES) & 1);
-        return;
-    }
-    for (uint32_t v = threadIdx.x; v < BM * (COLS / 8); v += kTileThreads) {
-        const uint32_t r = v / (COLS / 8), c = (v % (COLS / 8)) * 8;
-        if (m0 + r >= M || n0 + c >= N) continue;
-        float f[8], g[8];
-        const float* src = stage + r * Cfg::LD + c;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = src[e];
-        if (Epi::kGated) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) g[e] = src[64 + e];
-        }
-        epi(m0 + r, n0 + c, f, g);
-    }
-}
-
 // A product C[M, N] = A[M, K] . B[K, N] with an epilogue.  a_mn: A is stored
 // [K, M]; b_mn: B is stored [K, nb] (else [nb, K]), of which a gated product
-// reads columns n and n + N for its output column n (nb = 2 N).
+// reads columns n and n + N for its output column n (nb = 2 N).  early: B is
+// an argument of the call and a kernel of the same call runs just before, so
+// B may be read while that one ends (linear_slab.cuh).  trigger: another
+// kernel of the same call follows and may start while this one ends; the
+// caller's next kernel may not, since it need not expect that.
 struct Product {
     const void *A, *B;
     uint32_t M, N, K, nb;
     bool b_mn;
     int dtype;
     cudaStream_t st;
+    bool early = false;
+    bool trigger = false;
 };
 
 // Sets a kernel's shared-memory limit once per device.
@@ -210,34 +53,67 @@ int allow_smem(K* kern, int bytes, std::atomic<uint64_t>& done) {
     return EVKCU_OK;
 }
 
-// Operand maps; box_b: rows of a box of B stored [nb, K].
+// Operand maps; box_a, box_b: rows of a box of A stored [M, K] and of B
+// stored [nb, K] (otherwise boxes are 64 columns of a K-row).
+constexpr uint32_t BK = 64;
 template <bool A_MN, bool B_MN>
-int operand_maps(const Product& p, CUtensorMap* ta, CUtensorMap* tb, uint32_t box_b) {
+int operand_maps(const Product& p, CUtensorMap* ta, CUtensorMap* tb, uint32_t box_a, uint32_t box_b) {
     EVKCU_TRY(A_MN ? make_tmap_3d(ta, p.A, p.M, p.K, 1, p.M, (uint64_t)p.M * p.K, 64, BK, p.dtype)
-                   : make_tmap_3d(ta, p.A, p.K, p.M, 1, p.K, (uint64_t)p.M * p.K, BK, BM, p.dtype));
+                   : make_tmap_3d(ta, p.A, p.K, p.M, 1, p.K, (uint64_t)p.M * p.K, BK, box_a, p.dtype));
     return B_MN ? make_tmap_3d(tb, p.B, p.nb, p.K, 1, p.nb, (uint64_t)p.nb * p.K, 64, BK, p.dtype)
                 : make_tmap_3d(tb, p.B, p.K, p.nb, 1, p.K, (uint64_t)p.nb * p.K, BK, box_b, p.dtype);
 }
 
-template <typename T, int BN, bool A_MN, bool B_MN, class Epi>
-int launch_tile(const Product& p, const Epi& epi) {
-    using Cfg = TileCfg<BN>;
-    CUtensorMap ta, tb;
-    EVKCU_TRY((operand_maps<A_MN, B_MN>(p, &ta, &tb, 64)));
-    auto kern = tile_kernel<T, BN, A_MN, B_MN, Epi>;
-    static std::atomic<uint64_t> done{0};
-    EVKCU_TRY(allow_smem(kern, Cfg::SMEM, done));
-    constexpr uint32_t COLS = Epi::kGated ? BN / 2 : BN;
-    const dim3 grid((p.N + COLS - 1) / COLS, (p.M + BM - 1) / BM);
-    const uint32_t idesc = make_idesc_f16(BM, BN, p.dtype == EVKCU_BF16 ? 1 : 0, A_MN, B_MN);
-    kern<<<grid, kTileThreads, Cfg::SMEM, p.st>>>(ta, tb, epi, p.M, p.N, p.K, p.N, idesc, state()->d_error);
-    return after_launch("evkcu_linear(tile)");
+// Splits of K for `tiles` slab tiles: one CTA per SM where that is possible
+// (16 x 14336 x 4096: 4 splits of 32 slabs 21.1 us, 8 23.8), else as many as
+// are resident; two k-blocks each at least.  A cluster of 8 packs badly where
+// a CTA takes an SM (64 x 8192 x 2048: 4 splits 14.1 us, 8 22.1).
+uint32_t slab_splits(int mr, uint64_t tiles, uint32_t kblocks, int sms) {
+    const uint64_t sm = (uint64_t)sms, slots = mr == 16 ? 2 * sm : sm;
+    const uint64_t most = mr == 16 ? 8 : 4, fit = tiles <= sm / 2 ? sm / tiles : slots / tiles;
+    return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({most, fit, (kblocks + 1) / 2}));
 }
 
-// The staged form of each epilogue: its boxes' maps (128 rows x 32 columns of
+template <typename T, int MR, bool A_MN, bool B_MN, class Epi>
+int launch_slab(const Product& p, const Epi& epi) {
+    using C = slabk::Cfg<MR>;
+    CUtensorMap tx, tw;
+    EVKCU_TRY((operand_maps<A_MN, B_MN>(p, &tx, &tw, MR, 64)));
+    auto kern = slabk::slab_kernel<T, MR, A_MN, B_MN, Epi>;
+    static std::atomic<uint64_t> done{0};
+    EVKCU_TRY(allow_smem(kern, C::SMEM, done));
+    DeviceState* ds = state();
+    const uint32_t out = Epi::kGated ? 64 : 128;
+    const uint32_t slabs = (p.N + out - 1) / out, tiles = (p.M + MR - 1) / MR, kblocks = (p.K + BK - 1) / BK;
+    EVKCU_CHECK_ARG(tiles <= 65535, EVKCU_BAD_SHAPE, "evkcu_linear: too many output tiles");
+    const uint32_t want = slab_splits(MR, (uint64_t)slabs * tiles, kblocks, ds->sm_count);
+    const uint32_t per = (kblocks + want - 1) / want;
+    const uint32_t splits = (kblocks + per - 1) / per;  // none of them empty
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(slabs, tiles, splits);
+    cfg.blockDim = dim3(slabk::THREADS);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = p.st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = splits;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = ds->pdl ? 2 : 1;
+    const uint32_t idesc = sm100::make_idesc_f16(128, MR, p.dtype == EVKCU_BF16 ? 1 : 0, B_MN, A_MN);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tx, tw, epi, p.M, p.N, p.K, per, idesc,
+                                             (int)(p.early && ds->pdl), (int)p.trigger, ds->d_error);
+    if (e != cudaSuccess) return cuda_fail(e, "evkcu_linear(slab)");
+    return after_launch("evkcu_linear(slab)");
+}
+
+// The staged form of each epilogue: its boxes' maps (32 rows x 32 columns of
 // a [M, N] matrix with rows of `pitch` elements) and parameters.
 int box_map(CUtensorMap* m, const void* p, const Product& pr, uint64_t pitch) {
-    return make_tmap_3d(m, p, pr.N, pr.M, 1, pitch, pitch * pr.M, 32, 128, pr.dtype, 64);
+    return make_tmap_3d(m, p, pr.N, pr.M, 1, pitch, pitch * pr.M, 32, 32, pr.dtype, 64);
 }
 template <typename T>
 int stage(const Product& p, const EpiLinear<T>& e, pairk::Maps& m, pairk::StagedLinear<T>& s) {
@@ -248,40 +124,38 @@ int stage(const Product& p, const EpiLinear<T>& e, pairk::Maps& m, pairk::Staged
 }
 template <typename T>
 int stage(const Product& p, const EpiGated<T>& e, pairk::Maps& m, pairk::StagedGated<T>& s) {
-    s = pairk::StagedGated<T>{e.act, e.pre != nullptr};
-    if (e.pre) {
-        EVKCU_TRY(box_map(&m.out1, e.pre, p, 2 * (uint64_t)p.N));
-        EVKCU_TRY(box_map(&m.out2, e.pre + p.N, p, 2 * (uint64_t)p.N));
-    }
-    return box_map(&m.out0, e.h, p, p.N);
+    s = pairk::StagedGated<T>{e.h, e.F, e.act, e.pre != nullptr};
+    if (!e.pre) return box_map(&m.out0, e.h, p, p.N);
+    EVKCU_TRY(box_map(&m.out0, e.pre, p, 2 * (uint64_t)p.N));
+    return box_map(&m.out1, e.pre + p.N, p, 2 * (uint64_t)p.N);
 }
 template <typename T>
 int stage(const Product& p, const EpiGatedBwd<T>& e, pairk::Maps& m, pairk::StagedGatedBwd<T>& s) {
-    s = pairk::StagedGatedBwd<T>{e.act, e.h != nullptr};
+    s = pairk::StagedGatedBwd<T>{e.h, e.F, e.act};
     const uint64_t pitch = 2 * (uint64_t)p.N;
     EVKCU_TRY(box_map(&m.in0, e.pre, p, pitch));
     EVKCU_TRY(box_map(&m.in1, e.pre + p.N, p, pitch));
     EVKCU_TRY(box_map(&m.out0, e.dpre, p, pitch));
-    EVKCU_TRY(box_map(&m.out1, e.dpre + p.N, p, pitch));
-    return e.h ? box_map(&m.out2, e.h, p, p.N) : (int)EVKCU_OK;
+    return box_map(&m.out1, e.dpre + p.N, p, pitch);
 }
 template <class Epi> struct StagedOf;
 template <typename T> struct StagedOf<EpiLinear<T>> { using type = pairk::StagedLinear<T>; };
 template <typename T> struct StagedOf<EpiGated<T>> { using type = pairk::StagedGated<T>; };
 template <typename T> struct StagedOf<EpiGatedBwd<T>> { using type = pairk::StagedGatedBwd<T>; };
 
-template <typename T, bool A_MN, bool B_MN, class Epi>
+template <typename T, int NB, bool A_MN, bool B_MN, class Epi>
 int launch_pair(const Product& p, const Epi& epi) {
     using S = typename StagedOf<Epi>::type;
+    using C = pairk::Cfg<NB>;
     DeviceState* ds = state();
-    auto kern = pairk::pair_kernel<T, A_MN, B_MN, S>;
+    auto kern = pairk::pair_kernel<T, NB, A_MN, B_MN, S>;
     static std::atomic<uint64_t> done{0};
-    EVKCU_TRY(allow_smem(kern, pairk::SMEM, done));
+    EVKCU_TRY(allow_smem(kern, C::SMEM, done));
     if (!ds->linear_clusters) {  // equal for every instantiation: one CTA per SM
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(2 * (ds->sm_count / 2));
         cfg.blockDim = dim3(pairk::THREADS);
-        cfg.dynamicSmemBytes = pairk::SMEM;
+        cfg.dynamicSmemBytes = C::SMEM;
         int n = 0;
         EVKCU_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
         ds->linear_clusters = std::max(n, 1);
@@ -289,23 +163,54 @@ int launch_pair(const Product& p, const Epi& epi) {
     pairk::Maps maps;
     memset(&maps, 0, sizeof(maps));
     S s;
-    EVKCU_TRY((operand_maps<A_MN, B_MN>(p, &maps.a, &maps.b, 128)));
+    EVKCU_TRY((operand_maps<A_MN, B_MN>(p, &maps.a, &maps.b, 128, NB)));
     EVKCU_TRY(stage(p, epi, maps, s));
-    constexpr uint64_t COLS = Epi::kGated ? 128 : 256;
+    constexpr uint64_t COLS = Epi::kGated ? NB : 2 * NB;
     const uint64_t tiles = ((uint64_t)p.M + 255) / 256 * ((p.N + COLS - 1) / COLS);
     EVKCU_CHECK_ARG(tiles <= 0xFFFFFFFFu / 2, EVKCU_BAD_SHAPE, "evkcu_linear: too many output tiles");
     const uint32_t grid = 2 * (uint32_t)std::min<uint64_t>(tiles, (uint64_t)ds->linear_clusters);
-    const uint32_t idesc = make_idesc_f16(256, 256, p.dtype == EVKCU_BF16 ? 1 : 0, A_MN, B_MN);
-    kern<<<grid, pairk::THREADS, pairk::SMEM, p.st>>>(maps, s, p.M, p.N, p.K, idesc, ds->d_error);
-    return after_launch("evkcu_linear(pair)");
+    const uint32_t idesc = sm100::make_idesc_f16(256, 2 * NB, p.dtype == EVKCU_BF16 ? 1 : 0, A_MN, B_MN);
+    return launch_pdl("evkcu_linear(pair)", kern, dim3(grid), dim3(pairk::THREADS), C::SMEM, p.st, maps, s, p.M, p.N,
+                      p.K, idesc, (int)p.trigger, ds->d_error);
 }
 
+// Which kernel a product takes: the least estimated time.  The estimates are
+// a start-and-finish cost plus rounds of tiles times k-blocks, in us (a slab CTA
+// works on one tile, so each of its rounds starts and finishes), fitted to graph-replayed runs of bf16 products with operands from HBM:
+//   M x K x N            pair 128   pair 64   slab 128 / 64   taken
+//   4096 x 2048 x 8192     90.4      104.3         -          pair 128
+//   2048 x 2048 x 2048     15.7       16.8       26.4         pair 128
+//   1024 x 2048 x 2048     15.2       11.1       13.8         pair 64
+//    333 x  512 x 1368      7.6        5.8        7.2         pair 64
+//    512 x 8192 x 2048     41.8       27.6       23.9         slab 128
+//     32 x 4096 x 14336    26.1       30.4       20.3         slab 64
+//    512 x 16384 x 512     76.9       47.4       22.2         slab 64
+//   2048 x   64 x 8192     13.2       14.3       35.0         pair 128
+// Up to 16 rows W is read once and multiplied by little: always the slab.
 template <typename T, bool A_MN, bool B_MN, class Epi>
 int launch_product(const Product& p, const Epi& epi) {
-    constexpr uint64_t COLS = Epi::kGated ? 128 : 256;
-    const uint64_t pair_tiles = ((uint64_t)p.M + 255) / 256 * ((p.N + COLS - 1) / COLS);
-    if (pair_tiles >= 40) return launch_pair<T, A_MN, B_MN>(p, epi);
-    return launch_tile<T, 128, A_MN, B_MN>(p, epi);
+    const int sms = state()->sm_count;
+    const uint32_t per = Epi::kGated ? 2 : 1;  // accumulator columns per output column
+    const double kb = (p.K + BK - 1) / BK;
+    auto tiles = [&](uint64_t rows, uint64_t cols) {
+        return (p.M + rows - 1) / rows * ((p.N * (uint64_t)per + cols - 1) / cols);
+    };
+    auto pair_us = [&](uint64_t cols, double start, double block, double least) {
+        return start + (double)((tiles(256, cols) + sms / 2 - 1) / (sms / 2)) * std::max(block * kb, least);
+    };
+    auto slab_us = [&](int mr) {
+        const uint64_t t = tiles(mr, 128);
+        const uint32_t s = slab_splits(mr, t, (uint32_t)kb, sms);
+        return (s > 1 ? 2.0 : 0.0) + (double)((t * s + sms - 1) / sms) * (4.6 + 0.27 * std::ceil(kb / s));
+    };
+    if constexpr (!A_MN) {
+        if (p.M <= 16) return launch_slab<T, 16, A_MN, B_MN>(p, epi);
+    }
+    const double wide = pair_us(256, 5.0, 0.285, 1.8), narrow = pair_us(128, 4.4, 0.18, 1.2);
+    const double s64 = slab_us(64), s128 = slab_us(128);
+    if (std::min(wide, narrow) <= std::min(s64, s128))
+        return wide <= narrow ? launch_pair<T, 128, A_MN, B_MN>(p, epi) : launch_pair<T, 64, A_MN, B_MN>(p, epi);
+    return s64 <= s128 ? launch_slab<T, 64, A_MN, B_MN>(p, epi) : launch_slab<T, 128, A_MN, B_MN>(p, epi);
 }
 
 // A transposed A (weight gradients) always comes with a B stored [K, nb].
@@ -366,19 +271,19 @@ __global__ void __cluster_dims__(1, kDactCluster, 1) __launch_bounds__(kDactThre
         for (int i = 0; i < 32; ++i) t += s_sum[i][threadIdx.x];
         s_col[threadIdx.x] = t;
     }
-    cluster_sync_all();
+    sm100::cluster_sync_all();
     const uint32_t c = blockIdx.x * 64 + threadIdx.x;
     if (blockIdx.y == 0 && threadIdx.x < 64 && c < N) {
         float t = acc ? Elem<T>::to_f(dbias[c]) : 0.0f;
         float part = 0.0f;
         for (uint32_t r = 0; r < kDactCluster; ++r) {
             float v;
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_shared_rank(&s_col[threadIdx.x], r)));
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(sm100::map_shared_rank(&s_col[threadIdx.x], r)));
             part += v;
         }
         dbias[c] = Elem<T>::from_f(t + part);
     }
-    cluster_sync_all();  // no CTA leaves while rank 0 still reads its sums
+    sm100::cluster_sync_all();  // no CTA leaves while rank 0 still reads its sums
 }
 
 template <typename T>
@@ -419,15 +324,17 @@ EpiLinear<T> epi_plain(void* y, uint32_t N, bool acc) {
 // dx[rows, K] (+)= dz[rows, N] . W^T, W [K, N] (or [N, K] when nk).
 template <typename T>
 int grad_input(const void* dz, const void* w, void* dx, uint32_t rows, uint32_t K, uint32_t N, bool nk, bool acc,
-               int dtype, cudaStream_t st) {
-    return product<T, false>(Product{dz, w, rows, K, N, K, nk, dtype, st}, epi_plain<T>(dx, K, acc));
+               int dtype, cudaStream_t st, bool early, bool trigger) {
+    return product<T, false>(Product{dz, w, rows, K, N, K, nk, dtype, st, early, trigger}, epi_plain<T>(dx, K, acc));
 }
 // dW[K, N] (+)= x^T dz (or its transpose [N, K] = dz^T x when nk).
 template <typename T>
 int grad_weight(const void* x, const void* dz, void* dw, uint32_t rows, uint32_t K, uint32_t N, bool nk, bool acc,
-                int dtype, cudaStream_t st) {
-    if (nk) return product<T, true>(Product{dz, x, N, K, rows, K, true, dtype, st}, epi_plain<T>(dw, K, acc));
-    return product<T, true>(Product{x, dz, K, N, rows, N, true, dtype, st}, epi_plain<T>(dw, N, acc));
+                int dtype, cudaStream_t st, bool trigger) {
+    if (nk)
+        return product<T, true>(Product{dz, x, N, K, rows, K, true, dtype, st, false, trigger},
+                                epi_plain<T>(dw, K, acc));
+    return product<T, true>(Product{x, dz, K, N, rows, N, true, dtype, st, false, trigger}, epi_plain<T>(dw, N, acc));
 }
 
 int zero_grad(void* p, uint64_t elems, bool acc, cudaStream_t st) {
@@ -491,8 +398,8 @@ extern "C" int evkcu_linear_backward(const void* x, const void* w, const void* p
     return EVKCU_DISPATCH_DTYPE(dtype, T, [&] {
         if (has_act || dbias) EVKCU_TRY(launch_dact<T>(dy, pre, dpre, dbias, rows, N, act, acc, st));
         const void* dz = has_act ? dpre : dy;
-        if (dx) EVKCU_TRY(grad_input<T>(dz, w, dx, rows, K, N, nk, acc, dtype, st));
-        if (dw) EVKCU_TRY(grad_weight<T>(x, dz, dw, rows, K, N, nk, acc, dtype, st));
+        if (dx) EVKCU_TRY(grad_input<T>(dz, w, dx, rows, K, N, nk, acc, dtype, st, has_act || dbias, dw != nullptr));
+        if (dw) EVKCU_TRY(grad_weight<T>(x, dz, dw, rows, K, N, nk, acc, dtype, st, false));
         return (int)EVKCU_OK;
     });
 }
@@ -519,10 +426,10 @@ extern "C" int evkcu_gated_ffn(const void* x, const void* w_in, const void* w_ou
     const bool nk = flags & EVKCU_MM_TRANSPOSE_B;
     cudaStream_t st = as_stream(stream);
     return EVKCU_DISPATCH_DTYPE(dtype, T, [&] {
-        EVKCU_TRY((product<T, false>(Product{x, w_in, rows, F, D, 2 * F, !nk, dtype, st},
+        EVKCU_TRY((product<T, false>(Product{x, w_in, rows, F, D, 2 * F, !nk, dtype, st, false, y != nullptr},
                                      EpiGated<T>{(T*)hidden, (T*)pre, F, act})));
         if (!y) return (int)EVKCU_OK;
-        return product<T, false>(Product{hidden, w_out, rows, D, F, D, !nk, dtype, st},
+        return product<T, false>(Product{hidden, w_out, rows, D, F, D, !nk, dtype, st, true},
                                  EpiLinear<T>{nullptr, (const T*)residual, (T*)y, nullptr, D, EVKCU_ACT_NONE});
     });
 }
@@ -557,11 +464,11 @@ extern "C" int evkcu_gated_ffn_backward(const void* x, const void* w_in, const v
                                out_span("dw_in", dw_in, D, 2 * (uint64_t)F), out_span("dw_out", dw_out, F, D)}));
     EVKCU_CHECK_ARG(state(), EVKCU_CUDA_ERROR, "evkcu_gated_ffn_backward: no device state");
     return EVKCU_DISPATCH_DTYPE(dtype, T, [&] {
-        EVKCU_TRY((product<T, false>(Product{dy, w_out, rows, F, D, F, nk, dtype, st},
+        EVKCU_TRY((product<T, false>(Product{dy, w_out, rows, F, D, F, nk, dtype, st, false, dx || dw_in || dw_out},
                                      EpiGatedBwd<T>{(const T*)pre, (T*)dpre, dw_out ? (T*)hidden : nullptr, F, act})));
-        if (dx) EVKCU_TRY(grad_input<T>(dpre, w_in, dx, rows, D, 2 * F, nk, acc, dtype, st));
-        if (dw_in) EVKCU_TRY(grad_weight<T>(x, dpre, dw_in, rows, D, 2 * F, nk, acc, dtype, st));
-        if (dw_out) EVKCU_TRY(grad_weight<T>(hidden, dy, dw_out, rows, F, D, nk, acc, dtype, st));
+        if (dx) EVKCU_TRY(grad_input<T>(dpre, w_in, dx, rows, D, 2 * F, nk, acc, dtype, st, true, dw_in || dw_out));
+        if (dw_in) EVKCU_TRY(grad_weight<T>(x, dpre, dw_in, rows, D, 2 * F, nk, acc, dtype, st, dw_out != nullptr));
+        if (dw_out) EVKCU_TRY(grad_weight<T>(hidden, dy, dw_out, rows, F, D, nk, acc, dtype, st, false));
         return (int)EVKCU_OK;
     });
 }

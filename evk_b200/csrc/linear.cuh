@@ -107,18 +107,20 @@ __device__ __forceinline__ void act_both(float z, int act, float& a, float& da) 
     }
 }
 
-// Eight values at once, the activation chosen outside the loop.
-__device__ __forceinline__ void act8(float (&f)[8], int act) {
+// All values of a chunk at once, the activation chosen outside the loop: a
+// branch per value costs more in instruction fetches than the function.
+template <int N>
+__device__ __forceinline__ void act_all(float (&f)[N], int act) {
     if (act == EVKCU_ACT_NONE) return;
     if (act == EVKCU_ACT_SILU) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = act_f(f[e], EVKCU_ACT_SILU);
+        for (int e = 0; e < N; ++e) f[e] = act_f(f[e], EVKCU_ACT_SILU);
     } else if (act == EVKCU_ACT_GELU) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = act_f(f[e], EVKCU_ACT_GELU);
+        for (int e = 0; e < N; ++e) f[e] = act_f(f[e], EVKCU_ACT_GELU);
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = act_f(f[e], EVKCU_ACT_RELU);
+        for (int e = 0; e < N; ++e) f[e] = act_f(f[e], EVKCU_ACT_RELU);
     }
 }
 
@@ -171,7 +173,7 @@ struct EpiLinear {
             for (int e = 0; e < 8; ++e) f[e] += t[e];
         }
         if (pre) st_vec8(pre + at, pack8<T>(f));
-        act8(f, act);
+        act_all(f, act);
         if (res) {
             unpack8<T>(ld_vec8(res + at), t);
 #pragma unroll
@@ -195,7 +197,7 @@ struct EpiGated {
             st_vec8(p, pack8<T>(g));
             st_vec8(p + F, pack8<T>(u));
         }
-        act8(g, act);
+        act_all(g, act);
 #pragma unroll
         for (int e = 0; e < 8; ++e) g[e] *= u[e];
         st_vec8(h + (uint64_t)row * F + col, pack8<T>(g));

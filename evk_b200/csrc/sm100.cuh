@@ -378,6 +378,18 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
 __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
+// The same barrier without memory ordering: for phases that only keep the
+// CTAs of a cluster alive, or whose data a fence has published.
+__device__ __forceinline__ void cluster_sync_relaxed() {
+    asm volatile("barrier.cluster.arrive.relaxed;\n\tbarrier.cluster.wait;" ::: "memory");
+}
+// Arrive on an mbarrier of any CTA of the cluster with nothing to publish but
+// the arrival (a tensor-memory buffer handed back after tcgen05.wait::ld).
+// Release at cluster scope waits for the thread's earlier stores: 600 clocks
+// on the CTA's own barrier, 1,500 on its pair's.
+__device__ __forceinline__ void mbar_arrive_relaxed(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
 // TMA load into this CTA's shared memory whose completion is counted on an
 // mbarrier of either CTA of the pair (`bar_cluster`, a shared::cluster
 // address).
