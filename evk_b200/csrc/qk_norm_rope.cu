@@ -9,11 +9,15 @@
 //
 // Bound by HBM: each value is read once and written once (backward: read x
 // and dy, write dx).  A group of LPH lanes holds one head in registers, eight
-// elements (16 bytes) a lane, so the mean is a few shuffles.  The angles of a
-// row are computed once per block into shared memory and serve all its heads.
+// elements (16 bytes) a lane, so the mean is a few shuffles.  A block's G =
+// 256 / LPH groups are GH heads x GR rows, and a group takes one head of U
+// rows at a time: the gain is loaded once for them and U (backward: 2 U)
+// 16-byte loads per lane are in flight.  The angles of a row are computed once
+// per block into shared memory, behind the first loads, and serve all heads.
 #include <algorithm>
 #include <cmath>
 #include <string>
+#include <type_traits>
 
 #include "linear.cuh"
 
@@ -21,6 +25,11 @@ namespace evkcu {
 namespace {
 
 constexpr int kThreads = 256;
+// Rows a group takes at a time, and resident blocks per SM.  Forward, 16384
+// rows of 32 heads of 128: 57 us; 2 rows and 5 blocks 65, 4 and 3 64, 4 and 5
+// 61, 1 and 8 77.  Backward, 8192 rows of 40: 67 us; 2 rows and 3 blocks 75,
+// 2 and 4 79.  (41 and 39 us at the copy rate; issue slots are 63 % busy.)
+constexpr int kFwdRows = 4, kFwdBlocks = 4, kBwdRows = 4, kBwdBlocks = 2;
 constexpr uint32_t kMaxHalf = 128;       // rotation pairs of the largest head (256)
 constexpr uint32_t kMaxPartials = 1024;  // gain-gradient partial rows in the workspace
 
@@ -32,8 +41,9 @@ struct QkArgs {
     uint32_t rows, S, H, Hk, Dh, rot;
     uint32_t pos_offset, cache_len;
     int half_split, cache;
-    float eps;
-    uint32_t R, heads_per_block;  // rows and heads of a block's tile
+    float eps, inv_dh;
+    uint32_t GH, GR;  // a block's groups: heads x rows (GH GR = G, powers of two)
+    uint32_t heads_per_block;
     // backward: gradients of the outputs come through (q, k)-shaped dqo, dko
     const void *dqo, *dko;
     uint64_t dqo_pitch, dko_pitch;
@@ -48,56 +58,76 @@ __device__ __forceinline__ int32_t position(const QkArgs& a, uint32_t row) {
 
 // (cos, sin) of pos * base^(-2 i / rot).  The angle is reduced to a fraction
 // of a turn in 64 bits: in 32 a position of 10^5 would leave it 0.004 off.
+// Within half a turn sin.approx and cos.approx are off by 2^-21 at most.
 __device__ __forceinline__ float2 turn_cs(double turns, int32_t pos) {
     const double t = (double)pos * turns;
-    float s, c;
-    sincospif(2.0f * (float)(t - rint(t)), &s, &c);
-    return make_float2(c, s);
+    const float x = 6.2831853071795865f * (float)(t - rint(t));
+    return make_float2(__cosf(x), __sinf(x));
+}
+
+// Row pitch of the angles: whole lanes of four pairs, the pairs past rot / 2
+// turned by 0 so that a lane need not look where the rotation ends.
+__host__ __device__ inline uint32_t angle_pitch(uint32_t rot) { return (rot / 2 + 3) / 4 * 4; }
+
+// The table lies among the kernel's parameters.  Lanes read different entries,
+// which the constant cache serves one at a time; by its generic address it
+// goes through L1.
+__device__ __forceinline__ double turns_at(const QkArgs& a, uint32_t p) {
+    double t;
+    asm("ld.f64 %0, [%1];" : "=d"(t) : "l"(&a.turns[p]));
+    return t;
 }
 
 __device__ __forceinline__ void fill_angles(const QkArgs& a, float2* cs, uint32_t row0, uint32_t nrows) {
-    const uint32_t half = a.rot / 2;
-    for (uint32_t i = threadIdx.x; i < nrows * half; i += kThreads)
-        cs[i] = turn_cs(a.turns[i % half], position(a, row0 + i / half));
+    const uint32_t pitch = angle_pitch(a.rot);
+    for (uint32_t i = threadIdx.x; i < nrows * pitch; i += kThreads) {
+        const uint32_t p = i % pitch;
+        cs[i] = p < a.rot / 2 ? turn_cs(turns_at(a, p), position(a, row0 + i / pitch)) : make_float2(1.0f, 0.0f);
+    }
 }
 
 // Rotates the lane's eight elements f (element c * 8 of the head on) by the
-// row's angles; sgn = -1 is the inverse rotation.  All lanes of the warp call
-// it together (half-split pairs exchange lanes c and c + rot / 16).
+// row's angles cs (16-byte aligned rows: see angle_pitch); sgn = -1 is the
+// inverse rotation.  All lanes of the warp call it together (half-split pairs
+// exchange lanes c and c + rot / 16).
 template <int LPH>
 __device__ __forceinline__ void rotate8(const QkArgs& a, const float2* cs, uint32_t c, float sgn, float (&f)[8]) {
     if (!a.half_split) {
+        if (c * 8 >= a.rot) return;
+        const float4* v = reinterpret_cast<const float4*>(cs + c * 4);
+        const float4 t0 = v[0], t1 = v[1];
+        const float co[4] = {t0.x, t0.z, t1.x, t1.z}, si[4] = {t0.y, t0.w, t1.y, t1.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const uint32_t p = c * 4 + j;
-            if (p < a.rot / 2) {
-                const float2 t = cs[p];
-                const float x = f[2 * j], y = f[2 * j + 1], s = sgn * t.y;
-                f[2 * j] = x * t.x - y * s;
-                f[2 * j + 1] = x * s + y * t.x;
-            }
+            const float x = f[2 * j], y = f[2 * j + 1], s = sgn * si[j];
+            f[2 * j] = x * co[j] - y * s;
+            f[2 * j + 1] = x * s + y * co[j];
         }
         return;
     }
     const uint32_t hl = a.rot / 16;  // lanes of one half
     const bool lo = c < hl, hi = !lo && c < 2 * hl;
-    const uint32_t partner = lo ? c + hl : (hi ? c - hl : c);
+    float o[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float o = __shfl_sync(0xffffffffu, f[e], partner, LPH);
-        if (lo || hi) {
-            const float2 t = cs[(lo ? c : c - hl) * 8 + e];
-            const float s = sgn * t.y;
-            f[e] = lo ? f[e] * t.x - o * s : o * s + f[e] * t.x;
-        }
+    for (int e = 0; e < 8; ++e) o[e] = __shfl_sync(0xffffffffu, f[e], lo ? c + hl : (hi ? c - hl : c), LPH);
+    if (!lo && !hi) return;
+    const float4* v = reinterpret_cast<const float4*>(cs + (lo ? c : c - hl) * 8);
+    const float s0 = lo ? -sgn : sgn;  // low half x cos - y sin, high half y cos + x sin
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float4 t = v[e];
+        f[2 * e] = f[2 * e] * t.x + s0 * o[2 * e] * t.y;
+        f[2 * e + 1] = f[2 * e + 1] * t.z + s0 * o[2 * e + 1] * t.w;
     }
 }
 
-template <int LPH>
-__device__ __forceinline__ float group_sum(float v) {
+// Sums over a group's lanes, U of them side by side.
+template <int LPH, int U>
+__device__ __forceinline__ void group_sums(float (&v)[U]) {
 #pragma unroll
-    for (int o = LPH / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o, LPH);
-    return v;
+    for (int o = LPH / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] += __shfl_xor_sync(0xffffffffu, v[u], o, LPH);
 }
 
 template <typename T>
@@ -106,51 +136,71 @@ __device__ __forceinline__ Vec8 load8(const void* p, uint64_t at, bool ok) {
     return ok ? ld_vec8(reinterpret_cast<const T*>(p) + at) : z;
 }
 
-template <typename T, int LPH>
-__global__ void __launch_bounds__(kThreads) qk_forward_kernel(const __grid_constant__ QkArgs a) {
-    extern __shared__ float2 s_cs[];  // [R][rot / 2]
-    constexpr uint32_t G = kThreads / LPH;
+// The lane's eight gains, or ones.
+template <typename T>
+__device__ __forceinline__ void load_gain(const void* gain, uint32_t c, bool lane_on, float (&w)[8]) {
+    if (gain) {
+        unpack8<T>(load8<T>(gain, c * 8, lane_on), w);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = 1.0f;
+}
+
+template <typename T, int LPH, int U>
+__global__ void __launch_bounds__(kThreads, kFwdBlocks) qk_forward_kernel(const __grid_constant__ QkArgs a) {
+    extern __shared__ __align__(16) float2 s_cs[];  // [GR U][angle_pitch]
     const uint32_t c = threadIdx.x % LPH, g = threadIdx.x / LPH;
+    const uint32_t gh = g % a.GH, gr = g / a.GH, half = angle_pitch(a.rot);
     const uint32_t total = a.H + a.Hk + (a.v ? a.Hk : 0);
-    const uint32_t h0 = blockIdx.y * a.heads_per_block, nh = min(a.heads_per_block, total - h0);
-    const uint32_t row0 = blockIdx.x * a.R, nrows = min(a.R, a.rows - row0);
-    fill_angles(a, s_cs, row0, nrows);
-    __syncthreads();
+    const uint32_t h_end = min(total, (blockIdx.y + 1) * a.heads_per_block);
+    const uint32_t R = a.GR * U, row0 = blockIdx.x * R, nrows = min(R, a.rows - row0);
     const bool lane_on = c * 8 < a.Dh;
-    for (uint32_t i0 = 0; i0 < nrows * nh; i0 += G) {
-        const uint32_t i = i0 + g;
-        const bool on = i < nrows * nh;
-        const uint32_t rl = on ? i / nh : 0, h = h0 + (on ? i % nh : 0), row = row0 + rl;
+    bool first = true;
+    for (uint32_t h0 = blockIdx.y * a.heads_per_block; h0 < h_end; h0 += a.GH) {
+        const uint32_t h = h0 + gh;
+        const bool on = h < h_end && lane_on;
         const bool is_q = h < a.H, is_v = h >= a.H + a.Hk;
         const uint32_t hk = is_q ? h : (is_v ? h - a.H - a.Hk : h - a.H);
         const void* src = is_q ? a.q : (is_v ? a.v : a.k);
         const uint64_t pitch = is_q ? a.q_pitch : (is_v ? a.v_pitch : a.k_pitch);
-        const bool ld = on && lane_on;
-        const Vec8 raw = load8<T>(src, row * pitch + (uint64_t)hk * a.Dh + c * 8, ld);
-        float f[8];
-        unpack8<T>(raw, f);
-        float ss = 0.0f;
+        const uint64_t col = (uint64_t)hk * a.Dh + c * 8;
+        Vec8 raw[U];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss += f[e] * f[e];
-        const float r = rsqrtf(group_sum<LPH>(ss) / (float)a.Dh + a.eps);
+        for (int u = 0; u < U; ++u) {
+            const uint32_t rl = gr + u * a.GR;
+            raw[u] = load8<T>(src, (row0 + rl) * pitch + col, on && rl < nrows);
+        }
         const void* gain = is_q ? a.gq : a.gk;
         float w[8];
-        if (gain) unpack8<T>(load8<T>(gain, c * 8, lane_on), w);
+        load_gain<T>(gain, c, lane_on, w);
+        if (first) {
+            fill_angles(a, s_cs, row0, nrows);
+            __syncthreads();
+            first = false;
+        }
+        void* dst = is_q ? a.qo : (is_v ? a.vo : a.ko);
+        const uint64_t opitch = is_q ? a.qo_pitch : a.ko_pitch;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = gain ? f[e] * r * w[e] : f[e] * r;
-        rotate8<LPH>(a, s_cs + rl * (a.rot / 2), c, 1.0f, f);
-        if (!ld) continue;
-        const Vec8 out = is_v ? raw : pack8<T>(f);
-        if (is_q) {
-            st_vec8(reinterpret_cast<T*>(a.qo) + row * a.qo_pitch + (uint64_t)h * a.Dh + c * 8, out);
-        } else {
+        for (int u = 0; u < U; ++u) {
+            const uint32_t rl = gr + u * a.GR, row = row0 + rl;
+            float f[8], ss[1] = {0.0f};
+            unpack8<T>(raw[u], f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss[0] += f[e] * f[e];
+            group_sums<LPH, 1>(ss);
+            const float r = rsqrtf(ss[0] * a.inv_dh + a.eps);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] *= r * w[e];
+            rotate8<LPH>(a, s_cs + min(rl, nrows - 1) * half, c, 1.0f, f);
+            bool st = on && rl < nrows;
             uint64_t at = row;
-            if (a.cache) {
+            if (a.cache && !is_q && st) {
                 const int32_t pos = position(a, row);
-                if (pos < 0 || (uint32_t)pos >= a.cache_len) continue;  // outside the cache: not stored
+                st = pos >= 0 && (uint32_t)pos < a.cache_len;  // outside the cache: not stored
                 at = (uint64_t)(row / a.S) * a.cache_len + (uint32_t)pos;
             }
-            st_vec8(reinterpret_cast<T*>(is_v ? a.vo : a.ko) + at * a.ko_pitch + (uint64_t)hk * a.Dh + c * 8, out);
+            if (st) st_vec8(reinterpret_cast<T*>(dst) + at * opitch + col, is_v ? raw[u] : pack8<T>(f));
         }
     }
 }
@@ -159,54 +209,80 @@ __global__ void __launch_bounds__(kThreads) qk_forward_kernel(const __grid_const
 // gain gradients over all heads it meets, the block adds its groups in order
 // and stores one partial row, and qk_gain_kernel adds the partials in order,
 // so the sums do not depend on timing.
-template <typename T, int LPH>
-__global__ void __launch_bounds__(kThreads) qk_backward_kernel(const __grid_constant__ QkArgs a) {
-    extern __shared__ float2 s_cs[];  // [R][rot / 2]; then the groups' sums [G][2][Dh]
+template <typename T, int LPH, int U>
+__global__ void __launch_bounds__(kThreads, kBwdBlocks) qk_backward_kernel(const __grid_constant__ QkArgs a) {
+    extern __shared__ __align__(16) float2 s_cs[];  // [GR U][angle_pitch]; then the groups' sums [G][2][Dh]
     constexpr uint32_t G = kThreads / LPH;
     const uint32_t c = threadIdx.x % LPH, g = threadIdx.x / LPH;
-    const uint32_t total = a.H + a.Hk;
+    const uint32_t gh = g % a.GH, gr = g / a.GH, half = angle_pitch(a.rot);
+    const uint32_t total = a.H + a.Hk, R = a.GR * U;
     const bool lane_on = c * 8 < a.Dh;
     float accq[8] = {}, acck[8] = {};
-    for (uint32_t row0 = blockIdx.x * a.R; row0 < a.rows; row0 += gridDim.x * a.R) {
-        const uint32_t nrows = min(a.R, a.rows - row0);
-        __syncthreads();  // the previous tile's angles have been read
-        fill_angles(a, s_cs, row0, nrows);
-        __syncthreads();
-        for (uint32_t i0 = 0; i0 < nrows * total; i0 += G) {
-            const uint32_t i = i0 + g;
-            const bool on = i < nrows * total;
-            const uint32_t rl = on ? i / total : 0, h = on ? i % total : 0, row = row0 + rl;
-            const bool is_q = h < a.H;
-            const uint32_t hk = is_q ? h : h - a.H;
-            const bool ld = on && lane_on;
-            const uint64_t col = (uint64_t)hk * a.Dh + c * 8;
-            float x[8], t[8];
-            unpack8<T>(load8<T>(is_q ? a.q : a.k, row * (is_q ? a.q_pitch : a.k_pitch) + col, ld), x);
-            unpack8<T>(load8<T>(is_q ? a.dqo : a.dko, row * (is_q ? a.dqo_pitch : a.dko_pitch) + col, ld), t);
-            float ss = 0.0f;
+    pdl_trigger();  // qk_gain_kernel, which waits for this one's end
+    for (uint32_t row0 = blockIdx.x * R; row0 < a.rows; row0 += gridDim.x * R) {
+        const uint32_t nrows = min(R, a.rows - row0);
+        bool first = true;
+        for (uint32_t h0 = 0; h0 < total; h0 += a.GH) {
+            const uint32_t h = h0 + gh;
+            const bool on = h < total && lane_on, is_q = h < a.H;
+            const uint64_t col = (uint64_t)(is_q ? h : h - a.H) * a.Dh + c * 8;
+            Vec8 rx[U], rt[U];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
-            const float r = rsqrtf(group_sum<LPH>(ss) / (float)a.Dh + a.eps);
-            rotate8<LPH>(a, s_cs + rl * (a.rot / 2), c, -1.0f, t);
+            for (int u = 0; u < U; ++u) {
+                const uint32_t rl = gr + u * a.GR, row = row0 + rl;
+                const bool ld = on && rl < nrows;
+                rx[u] = load8<T>(is_q ? a.q : a.k, row * (is_q ? a.q_pitch : a.k_pitch) + col, ld);
+                rt[u] = load8<T>(is_q ? a.dqo : a.dko, row * (is_q ? a.dqo_pitch : a.dko_pitch) + col, ld);
+            }
             const void* gain = is_q ? a.gq : a.gk;
             float w[8];
-            if (gain) unpack8<T>(load8<T>(gain, c * 8, lane_on), w);
-            float m = 0.0f;
+            load_gain<T>(gain, c, lane_on, w);
+            if (first) {
+                __syncthreads();  // the previous tile's angles have been read
+                fill_angles(a, s_cs, row0, nrows);
+                __syncthreads();
+                first = false;
+            }
+            float x[U][8], t[U][8], ss[U], m[U], acc[8] = {};
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                unpack8<T>(rx[u], x[u]);
+                unpack8<T>(rt[u], t[u]);
+                ss[u] = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) ss[u] += x[u][e] * x[u][e];
+            }
+            group_sums<LPH, U>(ss);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                rotate8<LPH>(a, s_cs + min(gr + u * a.GR, nrows - 1) * half, c, -1.0f, t[u]);
+                ss[u] = rsqrtf(ss[u] * a.inv_dh + a.eps);
+                m[u] = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[u][e] *= ss[u];  // n
+                    acc[e] += t[u][e] * x[u][e];
+                    t[u][e] *= w[e];  // dn
+                    m[u] += t[u][e] * x[u][e];
+                }
+            }
+            group_sums<LPH, U>(m);
+            T* dst = reinterpret_cast<T*>(is_q ? a.qo : a.ko) + col;
+            const uint64_t opitch = is_q ? a.qo_pitch : a.ko_pitch;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const uint32_t rl = gr + u * a.GR;
+                m[u] *= a.inv_dh;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) t[u][e] = ss[u] * (t[u][e] - x[u][e] * m[u]);
+                if (on && rl < nrows) st_vec8(dst + (row0 + rl) * opitch, pack8<T>(t[u]));
+            }
+            if (!a.partial) continue;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                x[e] *= r;  // n
-                const float d = t[e] * x[e];
-                if (is_q) accq[e] += d;
-                else acck[e] += d;
-                t[e] = gain ? t[e] * w[e] : t[e];  // dn
-                m += t[e] * x[e];
+                if (is_q) accq[e] += acc[e];
+                else acck[e] += acc[e];
             }
-            m = group_sum<LPH>(m) / (float)a.Dh;
-            if (!ld) continue;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) t[e] = r * (t[e] - x[e] * m);
-            T* dst = reinterpret_cast<T*>(is_q ? a.qo : a.ko) + row * (is_q ? a.qo_pitch : a.ko_pitch) + col;
-            st_vec8(dst, pack8<T>(t));
         }
     }
     if (!a.partial) return;
@@ -229,13 +305,20 @@ __global__ void __launch_bounds__(kThreads) qk_backward_kernel(const __grid_cons
 
 // dgain (+)= sum of the partial rows: 32 columns a block, 32 row lanes.
 template <typename T>
-__global__ void __launch_bounds__(1024) qk_gain_kernel(const float* __restrict__ partial, uint32_t n, uint32_t Dh,
+__global__ void __launch_bounds__(1024) qk_gain_kernel(const float* partial, uint32_t n, uint32_t Dh,
                                                        T* dgq, T* dgk, int acc) {
     __shared__ float s[32][33];
     const uint32_t lane = threadIdx.x & 31, rl = threadIdx.x >> 5, j = blockIdx.x * 32 + lane;
     float v = 0.0f;
-    if (j < 2 * Dh)
-        for (uint32_t i = rl; i < n; i += 32) v += partial[(uint64_t)i * 2 * Dh + j];
+    pdl_wait();
+    for (uint32_t i0 = rl; i0 < n; i0 += 32 * 8) {  // eight loads in flight, added in order
+        float t[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            t[k] = i0 + 32 * k < n && j < 2 * Dh ? partial[(uint64_t)(i0 + 32 * k) * 2 * Dh + j] : 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v += t[k];
+    }
     s[rl][lane] = v;
     __syncthreads();
     if (rl != 0 || j >= 2 * Dh) return;
@@ -258,6 +341,15 @@ int with_lph(uint32_t Dh, F&& f) {
         case 16: return f(std::integral_constant<int, 16>());
         default: return f(std::integral_constant<int, 32>());
     }
+}
+
+// Heads x rows of a block's groups: the most heads that leave under a
+// sixteenth of the groups without one (40 heads, 16 groups: 8 x 2).
+void set_groups(QkArgs& a, uint32_t total) {
+    const uint32_t G = kThreads / lanes_per_head(a.Dh);
+    for (a.GH = G; a.GH > 1; a.GH /= 2)
+        if (total * 16 >= (total + a.GH - 1) / a.GH * a.GH * 15) break;
+    a.GR = G / a.GH;
 }
 
 bool pitch_ok(uint64_t pitch, uint64_t cols) { return pitch >= cols && pitch % 8 == 0 && pitch <= (1ull << 40); }
@@ -306,6 +398,7 @@ void fill_args(QkArgs& a, const evkcu_qk_norm_rope_desc* d) {
     a.positions = d->positions;
     a.half_split = (d->flags & EVKCU_QK_HALF_SPLIT) ? 1 : 0;
     a.eps = d->eps;
+    a.inv_dh = 1.0f / (float)a.Dh;
     // base^(-2 i / rot) by repeated products: 128 roundings of 2^-53 at most.
     const double ratio = std::pow((double)d->base, -2.0 / (double)a.rot);
     double t = 0.15915494309189535;  // 1 / (2 pi)
@@ -357,13 +450,19 @@ extern "C" int evkcu_qk_norm_rope(const evkcu_qk_norm_rope_desc* d, const void* 
     a.cache = cache;
     a.cache_len = d->cache_len;
     const uint32_t total = a.H + a.Hk + (v ? a.Hk : 0);
-    a.R = 1;
-    a.heads_per_block = total;
+    set_groups(a, total);
+    // kFwdRows rows a group where that still fills the SMs twice over; otherwise
+    // (decode) one row a group and one round of heads a block.
+    const uint64_t rounds = (total + a.GH - 1) / a.GH;
+    const bool large = ((uint64_t)a.rows + a.GR * kFwdRows - 1) / (a.GR * kFwdRows) >= 2 * (uint64_t)ds->sm_count;
+    a.heads_per_block = large ? total : a.GH;
     return EVKCU_DISPATCH_DTYPE(dtype, T, [&] {
         return with_lph(a.Dh, [&](auto lph) {
-            const dim3 grid((a.rows + a.R - 1) / a.R, (total + a.heads_per_block - 1) / a.heads_per_block);
-            qk_forward_kernel<T, lph.value>
-                <<<grid, kThreads, a.R * (a.rot / 2) * sizeof(float2), as_stream(stream)>>>(a);
+            const uint32_t R = a.GR * (large ? kFwdRows : 1);
+            const dim3 grid((a.rows + R - 1) / R, large ? 1 : (uint32_t)rounds);
+            const size_t smem = R * angle_pitch(a.rot) * sizeof(float2);  // at most 32 KB
+            if (large) qk_forward_kernel<T, lph.value, kFwdRows><<<grid, kThreads, smem, as_stream(stream)>>>(a);
+            else qk_forward_kernel<T, lph.value, 1><<<grid, kThreads, smem, as_stream(stream)>>>(a);
             return after_launch("evkcu_qk_norm_rope");
         });
     });
@@ -420,19 +519,20 @@ extern "C" int evkcu_qk_norm_rope_backward(const evkcu_qk_norm_rope_desc* d, con
     a.q_pitch = d->q_pitch, a.k_pitch = d->k_pitch, a.dqo_pitch = d->q_out_pitch, a.dko_pitch = d->k_out_pitch;
     a.qo_pitch = d->dq_pitch, a.ko_pitch = d->dk_pitch;
     a.partial = gains ? (float*)workspace : nullptr;
-    a.R = 1;
+    set_groups(a, a.H + a.Hk);
     return EVKCU_DISPATCH_DTYPE(dtype, T, [&] {
         return with_lph(a.Dh, [&](auto lph) {
-            const uint32_t tiles = (a.rows + a.R - 1) / a.R;
-            const uint32_t grid = std::min({tiles, kMaxPartials, 4u * (uint32_t)ds->sm_count});
-            const size_t smem = std::max<size_t>(a.R * (a.rot / 2) * sizeof(float2),
+            constexpr uint32_t U = kBwdRows;
+            const uint32_t R = a.GR * U, tiles = (a.rows + R - 1) / R;
+            const uint32_t grid = std::min({tiles, kMaxPartials, kBwdBlocks * (uint32_t)ds->sm_count});  // resident at once
+            const size_t smem = std::max<size_t>(R * angle_pitch(a.rot) * sizeof(float2),
                                                  gains ? (size_t)(kThreads / lph.value) * 2 * a.Dh * sizeof(float) : 0);
-            qk_backward_kernel<T, lph.value><<<grid, kThreads, smem, st>>>(a);
+            qk_backward_kernel<T, lph.value, U><<<grid, kThreads, smem, st>>>(a);
             EVKCU_TRY(after_launch("evkcu_qk_norm_rope_backward"));
             if (!gains) return (int)EVKCU_OK;
-            qk_gain_kernel<T><<<(2 * a.Dh + 31) / 32, 1024, 0, st>>>(a.partial, grid, a.Dh, (T*)dgain_q, (T*)dgain_k,
-                                                                    acc);
-            return after_launch("evkcu_qk_norm_rope_backward(gains)");
+            return launch_pdl("evkcu_qk_norm_rope_backward(gains)", qk_gain_kernel<T>, dim3((2 * a.Dh + 31) / 32),
+                              dim3(1024), 0, st, (const float*)a.partial, grid, a.Dh, (T*)dgain_q, (T*)dgain_k,
+                              (int)acc);
         });
     });
 }
