@@ -156,7 +156,8 @@ def _stream(stream) -> int:
     import torch
 
     if stream is None:
-        return torch.cuda.current_stream().cuda_stream
+        # the raw handle, without building a Stream object (3 us a call)
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
     return getattr(stream, "cuda_stream", stream)
 
 
@@ -456,21 +457,23 @@ SIGNATURES.update({
 _RET["evkcu_qk_norm_rope_workspace"] = _u64
 
 
-def _same(op, like, shapes):
-    """Checks tensors (None allowed) against `like`'s dtype and device and the
-    wanted shapes: {name: (tensor, shape)}."""
+def _same(op, like, *want):
+    """Checks (name, tensor or None, shape) triples against `like`'s dtype and
+    device, which has to be the current one."""
     import torch
 
-    if like.is_cuda and like.get_device() != torch.cuda.current_device():
-        raise EvkcuError(op, 7, f"tensors are on cuda:{like.get_device()}, the current device is "
-                                f"cuda:{torch.cuda.current_device()}")
-    for name, (t, shape) in shapes.items():
+    dt, dev = like.dtype, like.get_device()
+    for i in range(0, len(want), 3):
+        t = want[i + 1]
         if t is None:
             continue
-        if t.dtype != like.dtype or t.device != like.device:
-            raise EvkcuError(op, 7, f"{name} is {t.dtype} on {t.device}, expected {like.dtype} on {like.device}")
-        if tuple(t.shape) != tuple(shape):
-            raise EvkcuError(op, 1, f"{name} is {tuple(t.shape)}, expected {tuple(shape)}")
+        if t.dtype != dt or t.get_device() != dev:
+            raise EvkcuError(op, 7, f"{want[i]} is {t.dtype} on {t.device}, expected {dt} on {like.device}")
+        if t.shape != want[i + 2]:
+            raise EvkcuError(op, 1, f"{want[i]} is {tuple(t.shape)}, expected {tuple(want[i + 2])}")
+    if dev >= 0 and dev != torch.cuda.current_device():
+        raise EvkcuError(op, 7, f"tensors are on cuda:{dev}, the current device is "
+                                f"cuda:{torch.cuda.current_device()}")
 
 
 def linear(x, w, y, bias=None, residual=None, act=ACT_NONE, pre=None, transpose_w=False, stream=None):
@@ -479,12 +482,11 @@ def linear(x, w, y, bias=None, residual=None, act=ACT_NONE, pre=None, transpose_
     x (..., K); w (K, N), or (N, K) with transpose_w; bias (N,); residual, y
     and pre (..., N), pre receiving x @ w + bias for linear_backward.  residual
     may be y."""
-    K = x.shape[-1]
+    *lead, K = x.shape
     N = y.shape[-1]
-    lead = tuple(x.shape[:-1])
-    out = lead + (N,)
-    _same("linear", x, dict(w=(w, (N, K) if transpose_w else (K, N)), y=(y, out), bias=(bias, (N,)),
-                            residual=(residual, out), pre=(pre, out)))
+    out = (*lead, N)
+    _same("linear", x, "w", w, (N, K) if transpose_w else (K, N), "y", y, out, "bias", bias, (N,), "residual",
+          residual, out, "pre", pre, out)
     _check("evkcu_linear", lib().evkcu_linear(
         _ptr(x), _ptr(w), _ptr(bias), _ptr(residual), _ptr(y), _ptr(pre), x.numel() // K if K else 0, K, N, act,
         MM_TRANSPOSE_B if transpose_w else 0, _dtype_code(x), _stream(stream)))
@@ -498,10 +500,10 @@ def linear_backward(x, w, dy, dx=None, dw=None, dbias=None, act=ACT_NONE, pre=No
     linear's and dpre (like pre; pre or dy itself is allowed) receives the
     gradient of x @ w + bias."""
     K, N = x.shape[-1], dy.shape[-1]
-    out = tuple(x.shape[:-1]) + (N,)
+    out = (*x.shape[:-1], N)
     wshape = (N, K) if transpose_w else (K, N)
-    _same("linear_backward", x, dict(w=(w, wshape), dy=(dy, out), dx=(dx, x.shape), dw=(dw, wshape),
-                                     dbias=(dbias, (N,)), pre=(pre, out), dpre=(dpre, out)))
+    _same("linear_backward", x, "w", w, wshape, "dy", dy, out, "dx", dx, x.shape, "dw", dw, wshape, "dbias", dbias,
+          (N,), "pre", pre, out, "dpre", dpre, out)
     flags = (MM_TRANSPOSE_B if transpose_w else 0) | (MM_ACC_C if acc else 0)
     _check("evkcu_linear_backward", lib().evkcu_linear_backward(
         _ptr(x), _ptr(w), _ptr(pre), _ptr(dy), _ptr(dpre), _ptr(dx), _ptr(dw), _ptr(dbias),
@@ -517,11 +519,10 @@ def gated_ffn(x, w_in, w_out, y, hidden, act=ACT_SILU, residual=None, pre=None, 
     with transpose_w; hidden (..., F); pre (..., 2 F) receives [g | u] for
     gated_ffn_backward.  y = None (then w_out may be None) stops at hidden."""
     D, F = x.shape[-1], hidden.shape[-1]
-    lead = tuple(x.shape[:-1])
-    _same("gated_ffn", x, dict(w_in=(w_in, (2 * F, D) if transpose_w else (D, 2 * F)),
-                               w_out=(w_out, (D, F) if transpose_w else (F, D)), y=(y, x.shape),
-                               hidden=(hidden, lead + (F,)), residual=(residual, x.shape),
-                               pre=(pre, lead + (2 * F,))))
+    lead = x.shape[:-1]
+    _same("gated_ffn", x, "w_in", w_in, (2 * F, D) if transpose_w else (D, 2 * F), "w_out", w_out,
+          (D, F) if transpose_w else (F, D), "y", y, x.shape, "hidden", hidden, (*lead, F), "residual", residual,
+          x.shape, "pre", pre, (*lead, 2 * F))
     _check("evkcu_gated_ffn", lib().evkcu_gated_ffn(
         _ptr(x), _ptr(w_in), _ptr(w_out), _ptr(residual), _ptr(y), _ptr(hidden), _ptr(pre),
         x.numel() // D if D else 0, D, F, act, MM_TRANSPOSE_B if transpose_w else 0, _dtype_code(x),
@@ -536,12 +537,11 @@ def gated_ffn_backward(x, w_in, w_out, pre, dy, dpre, hidden, dx=None, dw_in=Non
     dpre (like pre; pre itself is allowed) receives its gradient; hidden
     (..., F) is recomputed and needed only for dw_out."""
     D, F = x.shape[-1], pre.shape[-1] // 2
-    lead = tuple(x.shape[:-1])
+    lead = x.shape[:-1]
     si, so = ((2 * F, D), (D, F)) if transpose_w else ((D, 2 * F), (F, D))
-    _same("gated_ffn_backward", x, dict(w_in=(w_in, si), w_out=(w_out, so), pre=(pre, lead + (2 * F,)),
-                                        dy=(dy, x.shape), dpre=(dpre, lead + (2 * F,)),
-                                        hidden=(hidden, lead + (F,)), dx=(dx, x.shape), dw_in=(dw_in, si),
-                                        dw_out=(dw_out, so)))
+    _same("gated_ffn_backward", x, "w_in", w_in, si, "w_out", w_out, so, "pre", pre, (*lead, 2 * F), "dy", dy,
+          x.shape, "dpre", dpre, (*lead, 2 * F), "hidden", hidden, (*lead, F), "dx", dx, x.shape, "dw_in", dw_in, si,
+          "dw_out", dw_out, so)
     flags = (MM_TRANSPOSE_B if transpose_w else 0) | (MM_ACC_C if acc else 0)
     _check("evkcu_gated_ffn_backward", lib().evkcu_gated_ffn_backward(
         _ptr(x), _ptr(w_in), _ptr(w_out), _ptr(pre), _ptr(dy), _ptr(dpre), _ptr(hidden), _ptr(dx), _ptr(dw_in),
@@ -549,43 +549,38 @@ def gated_ffn_backward(x, w_in, w_out, pre, dy, dpre, hidden, dx=None, dw_in=Non
     return dx, dw_in, dw_out
 
 
-def _rows(op, name, t, B, S, cols=None):
+def _rows(op, name, t, B, S):
     """(pointer, row pitch) of a (B, S, cols) tensor whose rows are evenly
     spaced (a slice of the last dimension of a contiguous tensor is)."""
     if not t.is_cuda:
         raise ValueError("evk_b200 ops take CUDA tensors")
-    if t.dim() != 3 or t.shape[0] != B or t.shape[1] != S or (cols is not None and t.shape[2] != cols):
-        raise EvkcuError(op, 1, f"{name} is {tuple(t.shape)}, expected {(B, S, cols)}")
     sb, st, sc = t.stride()
-    pitch = st if S > 1 else sb if B > 1 else max(t.shape[2], 1)
-    if (t.shape[2] > 1 and sc != 1) or (B > 1 and S > 1 and sb != S * st):
+    if (sc != 1 and t.shape[2] > 1) or (B > 1 and S > 1 and sb != S * st):
         raise EvkcuError(op, 1, f"{name}: strides {t.stride()} are not evenly spaced rows")
-    return t.data_ptr(), pitch
+    return t.data_ptr(), st if S > 1 else sb if B > 1 else max(t.shape[2], 1)
 
 
-def _qk_desc(op, q, k, heads, q_out, k_out, positions, rot_dim, half_split, eps, base, pos_offset):
-    import torch
-
+def _qk_shape(op, q, k, heads, positions, rot_dim, pos_offset):
+    """(B, S, head_dim, key columns, positions pointer) from q and k."""
     if q.dim() != 3 or heads <= 0 or q.shape[2] % heads:
         raise EvkcuError(op, 1, f"q is {tuple(q.shape)}, expected (B, S, {heads} heads * head_dim)")
-    B, S = q.shape[:2]
-    dh = q.shape[2] // heads
-    kv = 0
+    B, S, cols = q.shape
+    dh = cols // heads
+    kc = 0
     if k is not None:
         if dh == 0 or k.dim() != 3 or k.shape[2] % dh:
             raise EvkcuError(op, 1, f"k is {tuple(k.shape)}, expected (B, S, kv_heads * {dh})")
-        kv = k.shape[2] // dh
+        kc = k.shape[2]
     pos = None
     if positions is not None:
-        if positions.dtype != torch.int32 or positions.numel() != B * S or positions.device != q.device:
+        import torch
+
+        if positions.dtype != torch.int32 or positions.numel() != B * S or positions.get_device() != q.get_device():
             raise EvkcuError(op, 1, f"positions must be {B * S} int32 values on {q.device}")
         pos = _ptr(positions)
     if not 0 <= rot_dim <= 0xFFFFFFFF or not 0 <= pos_offset <= 0xFFFFFFFF:
         raise EvkcuError(op, 1, "rot_dim and pos_offset must be non-negative")
-    d = QkNormRopeDesc(batch=B, seq_len=S, heads=heads, kv_heads=kv, head_dim=dh, rot_dim=rot_dim,
-                       flags=QK_HALF_SPLIT if half_split else 0, pos_offset=pos_offset, eps=eps, base=base,
-                       positions=pos)
-    return d, B, S, kv * dh
+    return B, S, dh, kc, pos
 
 
 def qk_norm_rope(q, k, q_out, k_out, heads: int, gain_q=None, gain_k=None, v=None, v_out=None, cache=False,
@@ -597,36 +592,41 @@ def qk_norm_rope(q, k, q_out, k_out, heads: int, gain_q=None, gain_k=None, v=Non
     only; rows may be slices of a fused QKV tensor.  gain_q, gain_k (Dh,).
     positions: B * S int32 values, else pos_offset + t.  With cache=True, k_out
     is a contiguous KV cache (B, cache_len, Hkv * Dh) and keys go to the rows of
-    their positions; v is copied along to v_out."""
+    their positions.  v, where given, is copied along to v_out, which is laid
+    out as k_out."""
     op = "qk_norm_rope"
-    d, B, S, kc = _qk_desc(op, q, k, heads, q_out, k_out, positions, rot_dim, half_split, eps, base, pos_offset)
-    dh = d.head_dim
-    _same(op, q, dict(q_out=(q_out, q.shape), k=(k, (B, S, kc)), gain_q=(gain_q, (dh,)), gain_k=(gain_k, (dh,)),
-                      v=(v, (B, S, kc))))
-    qp, d.q_pitch = _rows(op, "q", q, B, S)
-    qo, d.q_out_pitch = _rows(op, "q_out", q_out, B, S)
+    B, S, dh, kc, pos = _qk_shape(op, q, k, heads, positions, rot_dim, pos_offset)
+    cache_len = 0
+    if k is None:
+        if v is not None or v_out is not None or cache:
+            raise EvkcuError(op, 7, "v, v_out and cache need k")
+    elif cache:
+        if k_out.dim() != 3:
+            raise EvkcuError(op, 1, f"k_out is {tuple(k_out.shape)}, expected (B, cache_len, {kc})")
+        cache_len = k_out.shape[1]
+    ks = (B, S, kc)
+    os = (B, cache_len, kc) if cache else ks
+    _same(op, q, "q_out", q_out, q.shape, "gain_q", gain_q, (dh,), "gain_k", gain_k, (dh,), "k", k, ks, "k_out",
+          k_out if k is not None else None, os, "v", v, ks, "v_out", v_out, os)
+    qp, q_pitch = _rows(op, "q", q, B, S)
+    qo, qo_pitch = _rows(op, "q_out", q_out, B, S)
     kp = ko = vp = vo = None
+    k_pitch = ko_pitch = v_pitch = 0
     if k is not None:
-        kp, d.k_pitch = _rows(op, "k", k, B, S)
+        kp, k_pitch = _rows(op, "k", k, B, S)
         if cache:
-            if k_out.dim() != 3:
-                raise EvkcuError(op, 1, f"k_out is {tuple(k_out.shape)}, expected (B, cache_len, {kc})")
-            d.flags |= QK_CACHE
-            d.cache_len = k_out.shape[1]
-            d.k_out_pitch = kc
-            _same(op, q, dict(k_out=(k_out, (B, d.cache_len, kc)), v_out=(v_out, k_out.shape)))
-            ko, vo = _ptr(k_out), _ptr(v_out)
+            ko, vo, ko_pitch = _ptr(k_out), _ptr(v_out), kc
         else:
-            _same(op, q, dict(k_out=(k_out, (B, S, kc)), v_out=(v_out, (B, S, kc))))
-            ko, d.k_out_pitch = _rows(op, "k_out", k_out, B, S)
+            ko, ko_pitch = _rows(op, "k_out", k_out, B, S)
             if v_out is not None:
-                vo, vpitch = _rows(op, "v_out", v_out, B, S)
-                if vpitch != d.k_out_pitch:
+                vo, vo_pitch = _rows(op, "v_out", v_out, B, S)
+                if vo_pitch != ko_pitch:
                     raise EvkcuError(op, 1, "v_out must have the row pitch of k_out")
         if v is not None:
-            vp, d.v_pitch = _rows(op, "v", v, B, S)
-    elif v is not None or v_out is not None or cache:
-        raise EvkcuError(op, 7, "v, v_out and cache need k")
+            vp, v_pitch = _rows(op, "v", v, B, S)
+    d = QkNormRopeDesc(B, S, heads, kc // dh if kc else 0, dh, rot_dim,
+                       (QK_HALF_SPLIT if half_split else 0) | (QK_CACHE if cache else 0), pos_offset, cache_len, eps,
+                       base, pos, q_pitch, k_pitch, v_pitch, qo_pitch, ko_pitch)
     _check("evkcu_qk_norm_rope", lib().evkcu_qk_norm_rope(
         d, qp, kp, vp, _ptr(gain_q), _ptr(gain_k), qo, ko, vo, _dtype_code(q), _stream(stream)))
     return q_out, k_out
@@ -646,26 +646,29 @@ def qk_norm_rope_backward(q, k, dq_out, dk_out, dq, dk, heads: int, gain_q=None,
     `workspace` tensor of qk_norm_rope_workspace(Dh) bytes and are added to with
     acc_gain."""
     op = "qk_norm_rope_backward"
-    d, B, S, kc = _qk_desc(op, q, k, heads, dq_out, dk_out, positions, rot_dim, half_split, eps, base, pos_offset)
-    dh = d.head_dim
-    _same(op, q, dict(dq_out=(dq_out, q.shape), dq=(dq, q.shape), gain_q=(gain_q, (dh,)), gain_k=(gain_k, (dh,)),
-                      dgain_q=(dgain_q, (dh,)), dgain_k=(dgain_k, (dh,))))
-    if acc_gain:
-        d.flags |= QK_ACC_GAIN
-    qp, d.q_pitch = _rows(op, "q", q, B, S)
-    gq, d.q_out_pitch = _rows(op, "dq_out", dq_out, B, S)
-    dqp, d.dq_pitch = _rows(op, "dq", dq, B, S)
+    B, S, dh, kc, pos = _qk_shape(op, q, k, heads, positions, rot_dim, pos_offset)
+    ks = (B, S, kc)
+    if k is None:
+        dk_out = dk = None
+    _same(op, q, "dq_out", dq_out, q.shape, "dq", dq, q.shape, "gain_q", gain_q, (dh,), "gain_k", gain_k, (dh,),
+          "dgain_q", dgain_q, (dh,), "dgain_k", dgain_k, (dh,), "k", k, ks, "dk_out", dk_out, ks, "dk", dk, ks)
+    qp, q_pitch = _rows(op, "q", q, B, S)
+    gq, gq_pitch = _rows(op, "dq_out", dq_out, B, S)
+    dqp, dq_pitch = _rows(op, "dq", dq, B, S)
     kp = gk = dkp = None
+    k_pitch = gk_pitch = dk_pitch = 0
     if k is not None:
-        _same(op, q, dict(k=(k, (B, S, kc)), dk_out=(dk_out, k.shape), dk=(dk, k.shape)))
-        kp, d.k_pitch = _rows(op, "k", k, B, S)
-        gk, d.k_out_pitch = _rows(op, "dk_out", dk_out, B, S)
-        dkp, d.dk_pitch = _rows(op, "dk", dk, B, S)
+        kp, k_pitch = _rows(op, "k", k, B, S)
+        gk, gk_pitch = _rows(op, "dk_out", dk_out, B, S)
+        dkp, dk_pitch = _rows(op, "dk", dk, B, S)
     wbytes = 0
     if workspace is not None:
-        if workspace.device != q.device:
+        if workspace.get_device() != q.get_device():
             raise EvkcuError(op, 7, f"workspace is on {workspace.device}, expected {q.device}")
         wbytes = workspace.numel() * workspace.element_size()
+    d = QkNormRopeDesc(B, S, heads, kc // dh if kc else 0, dh, rot_dim,
+                       (QK_HALF_SPLIT if half_split else 0) | (QK_ACC_GAIN if acc_gain else 0), pos_offset, 0, eps,
+                       base, pos, q_pitch, k_pitch, 0, gq_pitch, gk_pitch, dq_pitch, dk_pitch)
     _check("evkcu_qk_norm_rope_backward", lib().evkcu_qk_norm_rope_backward(
         d, qp, kp, _ptr(gain_q), _ptr(gain_k), gq, gk, dqp, dkp, _ptr(dgain_q), _ptr(dgain_k), _ptr(workspace), wbytes,
         _dtype_code(q), _stream(stream)))

@@ -354,7 +354,8 @@ void set_groups(QkArgs& a, uint32_t total) {
 
 bool pitch_ok(uint64_t pitch, uint64_t cols) { return pitch >= cols && pitch % 8 == 0 && pitch <= (1ull << 40); }
 
-int check_desc(const std::string& op, const evkcu_qk_norm_rope_desc* d, uint32_t allowed, int dtype) {
+int check_desc(const char* name, const evkcu_qk_norm_rope_desc* d, uint32_t allowed, int dtype) {
+    const std::string op(name);
     EVKCU_CHECK_ARG(d, EVKCU_BAD_ARG, op + ": descriptor is null");
     EVKCU_CHECK_ARG(dtype == EVKCU_F16 || dtype == EVKCU_BF16, EVKCU_BAD_ARG, op + ": unknown dtype");
     EVKCU_CHECK_ARG((d->flags & ~allowed) == 0, EVKCU_BAD_ARG, op + ": unknown flag");
@@ -375,15 +376,10 @@ int check_desc(const std::string& op, const evkcu_qk_norm_rope_desc* d, uint32_t
     return EVKCU_OK;
 }
 
-int check_tensor(const std::string& op, const char* name, const void* p, uint64_t pitch, uint64_t cols) {
-    EVKCU_CHECK_ARG(p, EVKCU_BAD_ARG, op + ": " + name + " is null");
-    EVKCU_CHECK_ARG(aligned16(p), EVKCU_BAD_ALIGN, op + ": " + name + " must be 16-byte aligned");
+int check_tensor(const char* op, const char* name, const void* p, uint64_t pitch, uint64_t cols) {
+    EVKCU_TRY(check_ptr(op, name, p, true));
     EVKCU_CHECK_ARG(pitch_ok(pitch, cols), EVKCU_BAD_SHAPE,
-                    op + ": the row pitch of " + name + " must be a multiple of 8 that holds its row");
-    return EVKCU_OK;
-}
-int check_gain(const std::string& op, const void* p) {
-    EVKCU_CHECK_ARG(aligned16(p), EVKCU_BAD_ALIGN, op + ": gains must be 16-byte aligned");
+                    std::string(op) + ": the row pitch of " + name + " must be a multiple of 8 that holds its row");
     return EVKCU_OK;
 }
 
@@ -430,8 +426,8 @@ extern "C" int evkcu_qk_norm_rope(const evkcu_qk_norm_rope_desc* d, const void* 
             EVKCU_TRY(check_tensor(op, "v_out", v_out, d->k_out_pitch, kc));
         }
     }
-    EVKCU_TRY(check_gain(op, gain_q));
-    EVKCU_TRY(check_gain(op, gain_k));
+    EVKCU_TRY(check_ptr(op, "gain_q", gain_q, false));
+    EVKCU_TRY(check_ptr(op, "gain_k", gain_k, false));
     const uint64_t rows = (uint64_t)d->batch * d->seq_len, krows = cache ? (uint64_t)d->batch * d->cache_len : rows;
     EVKCU_TRY(check_spans(op, {Span{"q", q, rows, d->q_pitch, qc}, Span{"k", k, rows, d->k_pitch, kc},
                                Span{"v", v, rows, d->v_pitch, kc}, Span{"gain_q", gain_q, 1, d->head_dim, d->head_dim},
@@ -480,8 +476,8 @@ extern "C" int evkcu_qk_norm_rope_backward(const evkcu_qk_norm_rope_desc* d, con
     EVKCU_TRY(check_desc(op, d, EVKCU_QK_HALF_SPLIT | EVKCU_QK_ACC_GAIN, dtype));
     const bool acc = d->flags & EVKCU_QK_ACC_GAIN, gains = dgain_q || dgain_k;
     cudaStream_t st = as_stream(stream);
-    EVKCU_TRY(check_gain(op, gain_q));
-    EVKCU_TRY(check_gain(op, gain_k));
+    EVKCU_TRY(check_ptr(op, "gain_q", gain_q, false));
+    EVKCU_TRY(check_ptr(op, "gain_k", gain_k, false));
     if ((uint64_t)d->batch * d->seq_len == 0) {  // empty sums
         if (dgain_q && !acc) EVKCU_CUDA_TRY(cudaMemsetAsync(dgain_q, 0, d->head_dim * 2, st));
         if (dgain_k && !acc) EVKCU_CUDA_TRY(cudaMemsetAsync(dgain_k, 0, d->head_dim * 2, st));
