@@ -205,52 +205,54 @@ __global__ void __launch_bounds__(THREADS, Cfg<MR>::PER_SM)
             mbar_drain(&full[i % STAGES], (i / STAGES) & 1);
     pdl_wait();  // before the epilogue reads or writes what earlier kernels may
     if (splits > 1) cluster_sync_all();
-    if (!*s_abort) {
-        const uint32_t rows = min((uint32_t)MR, M - m0);
-        const uint32_t base = smem_u32(stage);
-        const uint32_t vecs = rows * (OUT / 8);
-        if (splits == 1) {
-#pragma unroll 2
-            for (uint32_t v = threadIdx.x; v < vecs; v += THREADS) {
-                const uint32_t r = v / (OUT / 8), c = (v % (OUT / 8)) * 8;
-                const float* src = stage + r * LD + c;
-                float f[8], g[8];
+    // This CTA's share of the tile's rows, summed in place: nobody else reads
+    // these rows of its own partial.  A warp reads 512 consecutive bytes of
+    // each peer (16 of every 32 took twice as long), eight loads in flight.
+    const uint32_t rows = min((uint32_t)MR, M - m0), share = (rows + splits - 1) / splits;
+    const uint32_t r0 = split * share, r1 = min(rows, r0 + share);
+    if (splits > 1 && !*s_abort) {
+        constexpr uint32_t Q = COLS / 4;  // 16-byte pieces of a row
+        const uint32_t base = smem_u32(stage), n = r1 > r0 ? (r1 - r0) * Q : 0;
+        for (uint32_t i0 = threadIdx.x; i0 < n; i0 += 2 * THREADS) {
+            float sum[2][4] = {};
+            const uint32_t i1 = min(i0 + THREADS, n - 1);
+            const uint32_t at[2] = {base + ((r0 + i0 / Q) * LD + i0 % Q * 4) * 4,
+                                    base + ((r0 + i1 / Q) * LD + i1 % Q * 4) * 4};
+            for (uint32_t p0 = 0; p0 < splits; p0 += 4) {  // in rank order
+                float t[4][2][4];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] = src[e], g[e] = Epi::kGated ? src[64 + e] : 0.0f;
-                if (n0 + c < N) epi(m0 + r, n0 + c, f, g);
-            }
-        } else {
-            for (uint32_t v = split * THREADS + threadIdx.x; v < vecs; v += splits * THREADS) {
-                const uint32_t r = v / (OUT / 8), c = (v % (OUT / 8)) * 8;
-                float f[8] = {}, g[8] = {};
-                const uint32_t at = base + (r * LD + c) * 4;
-                // four CTAs' partials in flight at once, added in rank order
-                for (uint32_t p0 = 0; p0 < splits; p0 += 4) {
-                    float t[4][Epi::kGated ? 16 : 8];
+                for (int j = 0; j < 4; ++j) {
+                    if (p0 + j >= splits) continue;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (p0 + j >= splits) continue;
-                        uint32_t a;
-                        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(at), "r"(p0 + j));
-                        ld4_cluster(a, t[j]);
-                        ld4_cluster(a + 16, t[j] + 4);
-                        if constexpr (Epi::kGated) {
-                            ld4_cluster(a + 256, t[j] + 8);
-                            ld4_cluster(a + 272, t[j] + 12);
-                        }
-                    }
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (p0 + j >= splits) continue;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            f[e] += t[j][e];
-                            if constexpr (Epi::kGated) g[e] += t[j][8 + e];
-                        }
-                    }
+                    for (int k = 0; k < 2; ++k) ld4_cluster(map_shared_rank_u32(at[k], p0 + j), t[j][k]);
                 }
-                if (n0 + c < N) epi(m0 + r, n0 + c, f, g);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (p0 + j >= splits) continue;
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) sum[k][e] += t[j][k][e];
+                }
             }
+            float* dst = stage + (r0 + i0 / Q) * LD + i0 % Q * 4;
+            *reinterpret_cast<float4*>(dst) = make_float4(sum[0][0], sum[0][1], sum[0][2], sum[0][3]);
+            if (i0 + THREADS < n) {
+                dst = stage + (r0 + i1 / Q) * LD + i1 % Q * 4;
+                *reinterpret_cast<float4*>(dst) = make_float4(sum[1][0], sum[1][1], sum[1][2], sum[1][3]);
+            }
+        }
+        __syncthreads();
+    }
+    if (!*s_abort) {
+#pragma unroll 2
+        for (uint32_t v = r0 * (OUT / 8) + threadIdx.x; v < r1 * (OUT / 8); v += THREADS) {
+            const uint32_t r = v / (OUT / 8), c = (v % (OUT / 8)) * 8;
+            const float* src = stage + r * LD + c;
+            float f[8], g[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = src[e], g[e] = Epi::kGated ? src[64 + e] : 0.0f;
+            if (n0 + c < N) epi(m0 + r, n0 + c, f, g);
         }
     }
     if (splits > 1) cluster_sync_relaxed();  // no CTA leaves while its partial is read

@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) qk_backward_kernel(const
     const uint32_t total = a.H + a.Hk, R = a.GR * U;
     const bool lane_on = c * 8 < a.Dh;
     float accq[8] = {}, acck[8] = {};
-    pdl_trigger();  // qk_gain_kernel, which waits for this one's end
+    if (a.partial) pdl_trigger();  // qk_gain_kernel, which waits for this one to end
     for (uint32_t row0 = blockIdx.x * R; row0 < a.rows; row0 += gridDim.x * R) {
         const uint32_t nrows = min(R, a.rows - row0);
         bool first = true;

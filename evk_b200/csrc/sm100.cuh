@@ -331,10 +331,13 @@ __device__ __forceinline__ uint32_t cluster_count_x() {
     return r;
 }
 // Address of the same shared-memory offset in CTA `rank` of the cluster.
-__device__ __forceinline__ uint32_t map_shared_rank(const void* p, uint32_t rank) {
+__device__ __forceinline__ uint32_t map_shared_rank_u32(uint32_t addr, uint32_t rank) {
     uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
+}
+__device__ __forceinline__ uint32_t map_shared_rank(const void* p, uint32_t rank) {
+    return map_shared_rank_u32(smem_u32(p), rank);
 }
 // Arrive (release at cluster scope) on an mbarrier of another CTA.
 __device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
