@@ -56,4 +56,55 @@ void embed_ex(Tensor& embeddings, Tensor& indices, Tensor& out, uint32_t id_byte
 void greedy_sample_ex(Tensor& logits, Tensor& out_tokens, uint32_t position, uint32_t token_base,
                       uint32_t token_count, uint32_t id_bytes, DType dtype = DType::F16);
 
+// ---- decoder-layer operators around attention -------------------------------
+// The rules of include/evkcu.h hold (sizes in multiples of 8, which buffers
+// may coincide); optional tensors are pointers, nullptr for none.
+enum class Act : int { None = 0, Relu = 1, Gelu = 2, Silu = 3 };
+
+// y = act(x w + bias) + residual over the rows of x's last dimension; w is
+// (K, N), or (N, K) with transpose_w.  pre receives x w + bias.
+void linear(Tensor& x, Tensor& w, Tensor& y, Tensor* bias, Tensor* residual, Act act, Tensor* pre = nullptr,
+            bool transpose_w = false, DType dtype = DType::F16);
+// Gradients of linear from dy into those of dx, dw and dbias that are given,
+// or added to them with acc.  With an activation, pre is linear's and dpre
+// (like pre) receives its gradient.
+void linear_backward(Tensor& x, Tensor& w, Tensor& dy, Tensor* dx, Tensor* dw, Tensor* dbias, Act act,
+                     Tensor* pre = nullptr, Tensor* dpre = nullptr, bool transpose_w = false, bool acc = false,
+                     DType dtype = DType::F16);
+
+// Gated feed-forward block: [g | u] = x w_in, hidden = act(g) u, y = hidden
+// w_out + residual; w_in (D, 2 F), w_out (F, D), both transposed with
+// transpose_w.  pre (2 F a row) receives [g | u].
+void gated_ffn(Tensor& x, Tensor& w_in, Tensor& w_out, Tensor& y, Tensor& hidden, Act act, Tensor* residual = nullptr,
+               Tensor* pre = nullptr, bool transpose_w = false, DType dtype = DType::F16);
+// Its gradients from dy and the saved pre into those that are given; dpre
+// (like pre) receives pre's gradient, hidden is recomputed for dw_out.
+void gated_ffn_backward(Tensor& x, Tensor& w_in, Tensor& w_out, Tensor& pre, Tensor& dy, Tensor& dpre, Tensor& hidden,
+                        Tensor* dx, Tensor* dw_in, Tensor* dw_out, Act act, bool transpose_w = false,
+                        bool acc = false, DType dtype = DType::F16);
+
+// What qk_norm_rope rotates by, and how.
+struct QkRope {
+    uint32_t heads = 0;
+    uint32_t rot_dim = 0;     // rotated part of a head, 0 for all of it
+    bool half_split = false;  // pairs (i, i + rot_dim / 2) instead of (2 i, 2 i + 1)
+    uint32_t pos_offset = 0;  // position of token t: pos_offset + t
+    float eps = 1e-5f, base = 10000.0f;
+};
+
+// RMSNorm of every query and key head and its position rotation in one pass:
+// qkv (B, S, (heads + 2 Hkv) Dh) is a fused projection's output; q (B, S,
+// heads Dh), k and v (B, S, Hkv Dh) receive the queries, the keys and a copy
+// of the values.  With cached, k and v are caches (B, cache_len, Hkv Dh)
+// written at the tokens' positions.  gain_q, gain_k (Dh) or nullptr.
+void qk_norm_rope(Tensor& qkv, Tensor& q, Tensor& k, Tensor& v, Tensor* gain_q, Tensor* gain_k, const QkRope& rope,
+                  bool cached = false, DType dtype = DType::F16);
+// Its gradients: from dq, dk (as q and k without a cache) into the query and
+// key parts of dqkv (its value part is left as it is) and, where given,
+// dgain_q and dgain_k, which need a workspace of qk_norm_rope_workspace(Dh) bytes.
+void qk_norm_rope_backward(Tensor& qkv, Tensor& dq, Tensor& dk, Tensor& dqkv, Tensor* gain_q, Tensor* gain_k,
+                           Tensor* dgain_q, Tensor* dgain_k, Tensor* workspace, const QkRope& rope,
+                           DType dtype = DType::F16);
+uint64_t qk_norm_rope_workspace(uint32_t head_dim);
+
 }  // namespace evk::ai

@@ -13,11 +13,15 @@ Tolerances are bounds, element by element, with u = eps / 2 of the storage type
     wherever the value is not below the type's smallest step.
 """
 import math
+import os
+import subprocess
 
+import numpy as np
 import pytest
 import torch
 
 import evk_b200 as evk
+from conftest import ROOT, u16
 
 pytestmark = pytest.mark.gpu
 
@@ -739,3 +743,47 @@ def test_binding_refuses_mismatched_tensors():
         evk.qk_norm_rope(q, None, e(2, 3, 128), None, 3)
     with pytest.raises(evk.EvkcuError):
         evk.qk_norm_rope_backward(q, None, q, None, e(2, 3, 128), None, 2, dgain_q=e(64))  # no workspace
+
+
+LAYER = os.path.join(ROOT, "evk_b200", "reftests", "layer_check")
+
+
+@pytest.mark.skipif(not os.path.exists(LAYER), reason="layer_check not built")
+def test_cpp_layer_gives_the_bits_of_the_c_abi(tmp_path):
+    """evk_ai_ext.h's linear, gated_ffn and qk_norm_rope, forward and backward,
+    through libevk_ai.so (shapes in layer_check.cpp) against the same calls
+    through the Python binding: equal bits."""
+    dt, g = torch.bfloat16, gen(99)
+    B, S, D, F, H, Hk, dh = 2, 9, 256, 264, 4, 2, 64
+    C = (H + 2 * Hk) * dh
+    x, wqkv, bqkv = rnd(g, dt, B, S, D), rnd(g, dt, D, C, std=0.06), rnd(g, dt, C, std=0.1)
+    gq, gk = (rnd(g, dt, dh, std=0.1, mean=1.0) for _ in range(2))
+    wi, wo, dy = rnd(g, dt, D, 2 * F, std=0.06), rnd(g, dt, F, D, std=0.06), rnd(g, dt, B, S, D)
+    fin, fout = tmp_path / "in.bin", tmp_path / "out.bin"
+    fin.write_bytes(b"".join(u16(t).tobytes() for t in (x, wqkv, bqkv, gq, gk, wi, wo, dy)))
+    r = subprocess.run([LAYER, str(fin), str(fout)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "LAYER_OK" in r.stdout, (r.stdout + r.stderr)[-3000:]
+    e = lambda *s: torch.zeros(*s, dtype=dt, device="cuda")  # noqa: E731
+    qkv, q, k, v, kc, vc = e(B, S, C), e(B, S, D), e(B, S, 128), e(B, S, 128), e(B, 16, 128), e(B, 16, 128)
+    evk.linear(x, wqkv, qkv, bias=bqkv)
+    qi, ki, vi = qkv.split([H * dh, Hk * dh, Hk * dh], -1)
+    rope = dict(half_split=True, pos_offset=5)
+    evk.qk_norm_rope(qi, ki, q, k, H, gain_q=gq, gain_k=gk, v=vi, v_out=v, **rope)
+    evk.qk_norm_rope(qi, ki, q, kc, H, gain_q=gq, gain_k=gk, v=vi, v_out=vc, cache=True, **rope)
+    y, h, pre, dpre = e(B, S, D), e(B, S, F), e(B, S, 2 * F), e(B, S, 2 * F)
+    evk.gated_ffn(x, wi, wo, y, h, residual=x, pre=pre)
+    dx, dwi, dwo, dqkv = e(B, S, D), e(D, 2 * F), e(F, D), e(B, S, C)
+    evk.gated_ffn_backward(x, wi, wo, pre, dy, dpre, h, dx=dx, dw_in=dwi, dw_out=dwo)
+    dqi, dki, _ = dqkv.split([H * dh, Hk * dh, Hk * dh], -1)
+    dgq, dgk, dxq, dwqkv, dbqkv = e(dh), e(dh), e(B, S, D), e(D, C), e(C)
+    ws = torch.empty(evk.qk_norm_rope_workspace(dh), dtype=torch.uint8, device="cuda")
+    evk.qk_norm_rope_backward(qi, ki, q, k, dqi, dki, H, gain_q=gq, gain_k=gk, dgain_q=dgq, dgain_k=dgk, workspace=ws,
+                              **rope)
+    evk.linear_backward(x, wqkv, dqkv, dx=dxq, dw=dwqkv, dbias=dbqkv)
+    got, at = np.fromfile(fout, np.uint16), 0
+    names = "qkv q k v y pre dx dwi dwo dqkv dgq dgk dxq dwqkv dbqkv kc".split()
+    for name, t in zip(names, (qkv, q, k, v, y, pre, dx, dwi, dwo, dqkv, dgq, dgk, dxq, dwqkv, dbqkv, kc)):
+        want = u16(t).ravel()
+        assert np.array_equal(got[at:at + want.size], want), name
+        at += want.size
+    assert at == got.size
