@@ -223,75 +223,103 @@ int product(const Product& p, const Epi& epi) {
 }
 
 // -------------------------------- dz = dy act'(z) and its column sums ----
-// A cluster of 8 CTAs owns 64 columns; each CTA takes an eighth of the rows,
-// eight columns per thread, and keeps the column sums in registers.  They
-// are added across the CTA's 32 row lanes in shared memory, then across the
-// cluster in rank order over distributed shared memory: a fixed order and no
-// scratch in global memory.
+// A cluster of 8 CTAs owns 8 L columns; each CTA takes an eighth of the rows,
+// L lanes of eight columns a row, U rows of a lane in flight, and keeps the
+// column sums in registers.  They are added across the CTA's row lanes in
+// shared memory, then across the cluster in rank order over distributed shared
+// memory: a fixed order and no scratch in global memory.  dz may be dy or pre:
+// every element is read before it is written, by the same thread.
 constexpr uint32_t kDactCluster = 8;
 constexpr int kDactThreads = 256;
 
-template <typename T>
-__global__ void __cluster_dims__(1, kDactCluster, 1) __launch_bounds__(kDactThreads)
-    dact_kernel(const T* dy, const T* pre, T* dz, T* dbias, uint32_t rows, uint32_t N, int act, int acc) {
-    __shared__ float s_sum[32][64];
-    __shared__ float s_col[64];
-    const uint32_t cl = threadIdx.x & 7, rl = threadIdx.x >> 3;
-    const uint32_t col = blockIdx.x * 64 + cl * 8;
+template <typename T, int L, int U>
+__global__ void __cluster_dims__(1, kDactCluster, 1) __launch_bounds__(kDactThreads, U == 1 ? 8 : 3)
+    dact_kernel(const T* dy, const T* pre, T* dz, T* dbias, uint32_t rows, uint32_t N, int act, int acc,
+                int trigger) {
+    constexpr uint32_t RL = kDactThreads / L;  // row lanes
+    __shared__ float s_sum[RL][8 * L + 1];
+    __shared__ float s_col[8 * L];
+    const uint32_t cl = threadIdx.x % L, rl = threadIdx.x / L;
+    const uint32_t col = blockIdx.x * (8 * L) + cl * 8;
     const uint32_t per = (rows + kDactCluster - 1) / kDactCluster;
     const uint32_t r0 = blockIdx.y * per, r1 = min(rows, r0 + per);
     float sum[8] = {};
+    pdl_wait();
+    if (trigger) pdl_trigger();  // the product that follows; it waits for dz
     if (col < N) {
-#pragma unroll 4
-        for (uint32_t r = r0 + rl; r < r1; r += 32) {
-            const uint64_t at = (uint64_t)r * N + col;
-            float f[8];
-            unpack8<T>(ld_vec8(dy + at), f);
-            if (act != EVKCU_ACT_NONE) {
-                float z[8];
-                unpack8<T>(ld_vec8(pre + at), z);
+        for (uint32_t r = r0 + rl; r < r1; r += U * RL) {
+            Vec8 a[U], z[U];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    float a, da;
-                    act_both(z[e], act, a, da);
-                    f[e] *= da;
-                }
-                st_vec8(dz + at, pack8<T>(f));
+            for (int u = 0; u < U; ++u) {
+                const uint64_t at = (uint64_t)min(r + u * RL, r1 - 1) * N + col;
+                a[u] = ld_vec8(dy + at);
+                if (act != EVKCU_ACT_NONE) z[u] = ld_vec8(pre + at);
             }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) sum[e] += f[e];
+            for (int u = 0; u < U; ++u) {
+                if (r + u * RL >= r1) break;
+                float f[8];
+                unpack8<T>(a[u], f);
+                if (act != EVKCU_ACT_NONE) {
+                    float y[8];
+                    unpack8<T>(z[u], y);
+                    dact_all(f, y, act);
+                    st_vec8(dz + (uint64_t)(r + u * RL) * N + col, pack8<T>(f));
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum[e] += f[e];
+            }
         }
     }
     if (!dbias) return;
 #pragma unroll
     for (int e = 0; e < 8; ++e) s_sum[rl][cl * 8 + e] = sum[e];
     __syncthreads();
-    if (threadIdx.x < 64) {
+    for (uint32_t i = threadIdx.x; i < 8 * L; i += kDactThreads) {
         float t = 0.0f;
-        for (int i = 0; i < 32; ++i) t += s_sum[i][threadIdx.x];
-        s_col[threadIdx.x] = t;
+        for (uint32_t k = 0; k < RL; ++k) t += s_sum[k][i];
+        s_col[i] = t;
     }
     sm100::cluster_sync_all();
-    const uint32_t c = blockIdx.x * 64 + threadIdx.x;
-    if (blockIdx.y == 0 && threadIdx.x < 64 && c < N) {
-        float t = acc ? Elem<T>::to_f(dbias[c]) : 0.0f;
+    const uint32_t c = blockIdx.x * (8 * L) + threadIdx.x;
+    if (blockIdx.y == 0 && threadIdx.x < 8 * L && c < N) {
         float part = 0.0f;
         for (uint32_t r = 0; r < kDactCluster; ++r) {
             float v;
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(sm100::map_shared_rank(&s_col[threadIdx.x], r)));
+            asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                         : "=f"(v)
+                         : "r"(sm100::map_shared_rank(&s_col[threadIdx.x], r))
+                         : "memory");
             part += v;
         }
-        dbias[c] = Elem<T>::from_f(t + part);
+        if (acc) part += Elem<T>::to_f(dbias[c]);
+        dbias[c] = Elem<T>::from_f(part);
     }
-    sm100::cluster_sync_all();  // no CTA leaves while rank 0 still reads its sums
+    sm100::cluster_sync_relaxed();  // no CTA leaves while rank 0 still reads its sums
 }
 
+template <typename T, int L, int U>
+int launch_dact_of(const void* dy, const void* pre, void* dz, void* dbias, uint32_t rows, uint32_t N, int act, int acc,
+                   int trigger, cudaStream_t st) {
+    return launch_pdl("evkcu_linear_backward(dact)", dact_kernel<T, L, U>,
+                      dim3((N + 8 * L - 1) / (8 * L), kDactCluster), dim3(kDactThreads), 0, st, (const T*)dy,
+                      (const T*)pre, (T*)dz, (T*)dbias, rows, N, act, acc, trigger);
+}
+
+// One row a lane and eight CTAs an SM hide the memory best where there are
+// that many CTAs: 32 columns a cluster (4096 x 8192: 48 us; 64 columns 52,
+// four rows a lane and 64 columns 68), 16 in narrower layers (16384 x 2048:
+// 52 us against 63), and four rows a lane where even those are too few
+// (16384 x 512: 19 us against 28).
 template <typename T>
 int launch_dact(const void* dy, const void* pre, void* dz, void* dbias, uint32_t rows, uint32_t N, int act, int acc,
-                cudaStream_t st) {
-    dact_kernel<T><<<dim3((N + 63) / 64, kDactCluster), kDactThreads, 0, st>>>((const T*)dy, (const T*)pre, (T*)dz,
-                                                                              (T*)dbias, rows, N, act, acc);
-    return after_launch("evkcu_linear_backward(dact)");
+                int trigger, cudaStream_t st) {
+    const uint32_t enough = 5 * (uint32_t)state()->sm_count;
+    if ((N + 31) / 32 * kDactCluster >= enough)
+        return launch_dact_of<T, 4, 1>(dy, pre, dz, dbias, rows, N, act, acc, trigger, st);
+    if ((N + 15) / 16 * kDactCluster >= enough)
+        return launch_dact_of<T, 2, 1>(dy, pre, dz, dbias, rows, N, act, acc, trigger, st);
+    return launch_dact_of<T, 2, 4>(dy, pre, dz, dbias, rows, N, act, acc, trigger, st);
 }
 
 // ---------------------------------------------------------------- checks ----
@@ -396,7 +424,7 @@ extern "C" int evkcu_linear_backward(const void* x, const void* w, const void* p
                                out_span("dx", dx, rows, K), out_span("dw", dw, K, N), out_span("dbias", dbias, 1, N)}));
     EVKCU_CHECK_ARG(state(), EVKCU_CUDA_ERROR, "evkcu_linear_backward: no device state");
     return EVKCU_DISPATCH_DTYPE(dtype, T, [&] {
-        if (has_act || dbias) EVKCU_TRY(launch_dact<T>(dy, pre, dpre, dbias, rows, N, act, acc, st));
+        if (has_act || dbias) EVKCU_TRY(launch_dact<T>(dy, pre, dpre, dbias, rows, N, act, acc, dx || dw, st));
         const void* dz = has_act ? dpre : dy;
         if (dx) EVKCU_TRY(grad_input<T>(dz, w, dx, rows, K, N, nk, acc, dtype, st, has_act || dbias, dw != nullptr));
         if (dw) EVKCU_TRY(grad_weight<T>(x, dz, dw, rows, K, N, nk, acc, dtype, st, false));

@@ -107,6 +107,13 @@ __device__ __forceinline__ void act_both(float z, int act, float& a, float& da) 
     }
 }
 
+template <int ACT>
+__device__ __forceinline__ float dact_of(float z) {
+    float a, da;
+    act_both(z, ACT, a, da);
+    return da;
+}
+
 // All values of a chunk at once, the activation chosen outside the loop: a
 // branch per value costs more in instruction fetches than the function.
 template <int N>
@@ -121,6 +128,21 @@ __device__ __forceinline__ void act_all(float (&f)[N], int act) {
     } else {
 #pragma unroll
         for (int e = 0; e < N; ++e) f[e] = act_f(f[e], EVKCU_ACT_RELU);
+    }
+}
+
+// f *= act'(z)
+template <int N>
+__device__ __forceinline__ void dact_all(float (&f)[N], const float (&z)[N], int act) {
+    if (act == EVKCU_ACT_SILU) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] *= dact_of<EVKCU_ACT_SILU>(z[e]);
+    } else if (act == EVKCU_ACT_GELU) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] *= dact_of<EVKCU_ACT_GELU>(z[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] *= dact_of<EVKCU_ACT_RELU>(z[e]);
     }
 }
 
