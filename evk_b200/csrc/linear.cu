@@ -43,16 +43,6 @@ struct Product {
     bool trigger = false;
 };
 
-// Sets a kernel's shared-memory limit once per device.
-template <class K>
-int allow_smem(K* kern, int bytes, std::atomic<uint64_t>& done) {
-    const uint64_t bit = 1ull << (state()->device & 63);
-    if (done.load(std::memory_order_relaxed) & bit) return EVKCU_OK;
-    EVKCU_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    done.fetch_or(bit, std::memory_order_relaxed);
-    return EVKCU_OK;
-}
-
 // Operand maps; box_a, box_b: rows of a box of A stored [M, K] and of B
 // stored [nb, K] (otherwise boxes are 64 columns of a K-row).
 constexpr uint32_t BK = 64;

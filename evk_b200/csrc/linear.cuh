@@ -3,6 +3,7 @@
 // accumulators into outputs.
 #pragma once
 
+#include <atomic>
 #include <initializer_list>
 #include <string>
 
@@ -54,6 +55,16 @@ inline int check_spans(const char* op, std::initializer_list<Span> spans) {
             if (spans_overlap(*a, *b))
                 return fail(EVKCU_BAD_ARG, std::string(op) + ": " + a->name + " overlaps " + b->name);
         }
+    return EVKCU_OK;
+}
+
+// Sets a kernel's shared-memory limit once per device.
+template <class K>
+int allow_smem(K* kern, int bytes, std::atomic<uint64_t>& done) {
+    const uint64_t bit = 1ull << (state()->device & 63);
+    if (done.load(std::memory_order_relaxed) & bit) return EVKCU_OK;
+    EVKCU_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done.fetch_or(bit, std::memory_order_relaxed);
     return EVKCU_OK;
 }
 

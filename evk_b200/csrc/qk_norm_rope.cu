@@ -8,13 +8,14 @@
 //   dx = r (dn - n mean(dn * n))
 //
 // Bound by HBM: each value is read once and written once (backward: read x
-// and dy, write dx).  A group of LPH lanes holds one head in registers, eight
-// elements (16 bytes) a lane, so the mean is a few shuffles.  A block's G =
-// 256 / LPH groups are GH heads x GR rows, and a group takes one head of U
-// rows at a time: the gain is loaded once for them and U (backward: 2 U)
-// 16-byte loads per lane are in flight.  The angles of a row are computed once
-// per block into shared memory, behind the first loads, and serve all heads.
+// and dy, write dx), with the issue slots not far behind.  A group of LPH
+// lanes holds one head in registers, two vectors of eight elements a lane, so
+// the mean is three shuffles at 128.  A block's G = 256 / LPH groups are GH
+// heads x GR rows and walk its rows in rounds; asynchronous copies into the
+// thread's own slots of shared memory run ahead of them.  The angles of a row
+// are computed once per block into shared memory and serve all heads.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <string>
 #include <type_traits>
@@ -25,11 +26,14 @@ namespace evkcu {
 namespace {
 
 constexpr int kThreads = 256;
-// Rows a group takes at a time, and resident blocks per SM.  Forward, 16384
-// rows of 32 heads of 128: 57 us; 2 rows and 5 blocks 65, 4 and 3 64, 4 and 5
-// 61, 1 and 8 77.  Backward, 8192 rows of 40: 67 us; 2 rows and 3 blocks 75,
-// 2 and 4 79.  (41 and 39 us at the copy rate; issue slots are 63 % busy.)
-constexpr int kFwdRows = 4, kFwdBlocks = 4, kBwdRows = 4, kBwdBlocks = 2;
+// Rows a group takes in a round, rounds of copies ahead, and resident blocks
+// per SM.  Forward, 16384 rows of 32 heads of 128 (41 us at the copy rate):
+// 51 us; 3 rows 53, 5 rows 52, 2 rows and 2 ahead 59, 4 blocks 58 (spills).
+// Backward, 8192 rows of 40 heads (39 us): 57 us; 4 rows 61, 4 ahead 58,
+// 2 rows and 3 blocks 76 (spills).  One vector a lane (twice the lanes, a
+// shuffle more) took 55 and 63 us, loads through registers 57 and 67.
+constexpr int kFwdRows = 4, kFwdAhead = 1, kFwdBlocks = 3, kBwdRows = 1, kBwdAhead = 2, kBwdBlocks = 2;
+constexpr int kMaxSmem = 112 * 1024;     // slots and angles of a block
 constexpr uint32_t kMaxHalf = 128;       // rotation pairs of the largest head (256)
 constexpr uint32_t kMaxPartials = 1024;  // gain-gradient partial rows in the workspace
 
@@ -86,33 +90,21 @@ __device__ __forceinline__ void fill_angles(const QkArgs& a, float2* cs, uint32_
     }
 }
 
-// Rotates the lane's eight elements f (element c * 8 of the head on) by the
-// row's angles cs (16-byte aligned rows: see angle_pitch); sgn = -1 is the
-// inverse rotation.  All lanes of the warp call it together (half-split pairs
-// exchange lanes c and c + rot / 16).
-template <int LPH>
-__device__ __forceinline__ void rotate8(const QkArgs& a, const float2* cs, uint32_t c, float sgn, float (&f)[8]) {
-    if (!a.half_split) {
-        if (c * 8 >= a.rot) return;
-        const float4* v = reinterpret_cast<const float4*>(cs + c * 4);
-        const float4 t0 = v[0], t1 = v[1];
-        const float co[4] = {t0.x, t0.z, t1.x, t1.z}, si[4] = {t0.y, t0.w, t1.y, t1.w};
+// One vector of eight elements rotated by four (cos, sin) pairs.
+__device__ __forceinline__ void rotate_pairs(const float2* cs, float sgn, float (&f)[8]) {
+    const float4* v = reinterpret_cast<const float4*>(cs);
+    const float4 t0 = v[0], t1 = v[1];
+    const float co[4] = {t0.x, t0.z, t1.x, t1.z}, si[4] = {t0.y, t0.w, t1.y, t1.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float x = f[2 * j], y = f[2 * j + 1], s = sgn * si[j];
-            f[2 * j] = x * co[j] - y * s;
-            f[2 * j + 1] = x * s + y * co[j];
-        }
-        return;
+    for (int j = 0; j < 4; ++j) {
+        const float x = f[2 * j], y = f[2 * j + 1], s = sgn * si[j];
+        f[2 * j] = x * co[j] - y * s;
+        f[2 * j + 1] = x * s + y * co[j];
     }
-    const uint32_t hl = a.rot / 16;  // lanes of one half
-    const bool lo = c < hl, hi = !lo && c < 2 * hl;
-    float o[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = __shfl_sync(0xffffffffu, f[e], lo ? c + hl : (hi ? c - hl : c), LPH);
-    if (!lo && !hi) return;
-    const float4* v = reinterpret_cast<const float4*>(cs + (lo ? c : c - hl) * 8);
-    const float s0 = lo ? -sgn : sgn;  // low half x cos - y sin, high half y cos + x sin
+}
+// f = f cos + o s0 sin over eight (cos, sin) pairs.
+__device__ __forceinline__ void rotate_halves(const float2* cs, float s0, const float (&o)[8], float (&f)[8]) {
+    const float4* v = reinterpret_cast<const float4*>(cs);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const float4 t = v[e];
@@ -121,178 +113,287 @@ __device__ __forceinline__ void rotate8(const QkArgs& a, const float2* cs, uint3
     }
 }
 
-// Sums over a group's lanes, U of them side by side.
-template <int LPH, int U>
-__device__ __forceinline__ void group_sums(float (&v)[U]) {
+// Rotates the lane's two vectors, c and c + LPH of the head's, by the row's
+// angles cs (see angle_pitch); sgn = -1 is the inverse rotation.  All lanes of
+// the warp call it together: half-split pairs are vectors n and n + hl, the
+// lane's own two where hl = LPH, otherwise exchanged.
+template <int LPH>
+__device__ __forceinline__ void rotate(const QkArgs& a, const float2* cs, uint32_t c, float sgn, float (&f)[2][8]) {
+    if (!a.half_split) {
 #pragma unroll
-    for (int o = LPH / 2; o > 0; o >>= 1)
-#pragma unroll
-        for (int u = 0; u < U; ++u) v[u] += __shfl_xor_sync(0xffffffffu, v[u], o, LPH);
-}
-
-template <typename T>
-__device__ __forceinline__ Vec8 load8(const void* p, uint64_t at, bool ok) {
-    Vec8 z = {{0u, 0u, 0u, 0u}};
-    return ok ? ld_vec8(reinterpret_cast<const T*>(p) + at) : z;
-}
-
-// The lane's eight gains, or ones.
-template <typename T>
-__device__ __forceinline__ void load_gain(const void* gain, uint32_t c, bool lane_on, float (&w)[8]) {
-    if (gain) {
-        unpack8<T>(load8<T>(gain, c * 8, lane_on), w);
+        for (int v = 0; v < 2; ++v)
+            if ((c + v * LPH) * 8 < a.rot) rotate_pairs(cs + (c + v * LPH) * 4, sgn, f[v]);
         return;
     }
+    const uint32_t hl = a.rot / 16;
+    if (hl == LPH) {
+        float o[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = 1.0f;
+        for (int e = 0; e < 8; ++e) o[e] = f[0][e];
+        rotate_halves(cs + c * 8, -sgn, f[1], f[0]);  // low half: x cos - y sin
+        rotate_halves(cs + c * 8, sgn, o, f[1]);      // high half: y cos + x sin
+        return;
+    }
+    float o[2][8];
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+        const uint32_t n = c + v * LPH, at = n < hl ? n + hl : (n < 2 * hl ? n - hl : n);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            o[v][e] = __shfl_sync(0xffffffffu, f[0][e], at % LPH, LPH);
+            if (2 * hl > LPH) {  // the pair reaches into the second vectors
+                const float p = __shfl_sync(0xffffffffu, f[1][e], at % LPH, LPH);
+                if (at >= LPH) o[v][e] = p;
+            }
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+        const uint32_t n = c + v * LPH;
+        if (n < 2 * hl) rotate_halves(cs + (n < hl ? n : n - hl) * 8, n < hl ? -sgn : sgn, o[v], f[v]);
+    }
 }
 
-template <typename T, int LPH, int U>
-__global__ void __launch_bounds__(kThreads, kFwdBlocks) qk_forward_kernel(const __grid_constant__ QkArgs a) {
-    extern __shared__ __align__(16) float2 s_cs[];  // [GR U][angle_pitch]
-    const uint32_t c = threadIdx.x % LPH, g = threadIdx.x / LPH;
-    const uint32_t gh = g % a.GH, gr = g / a.GH, half = angle_pitch(a.rot);
-    const uint32_t total = a.H + a.Hk + (a.v ? a.Hk : 0);
-    const uint32_t h_end = min(total, (blockIdx.y + 1) * a.heads_per_block);
-    const uint32_t R = a.GR * U, row0 = blockIdx.x * R, nrows = min(R, a.rows - row0);
-    const bool lane_on = c * 8 < a.Dh;
-    bool first = true;
-    for (uint32_t h0 = blockIdx.y * a.heads_per_block; h0 < h_end; h0 += a.GH) {
-        const uint32_t h = h0 + gh;
-        const bool on = h < h_end && lane_on;
-        const bool is_q = h < a.H, is_v = h >= a.H + a.Hk;
-        const uint32_t hk = is_q ? h : (is_v ? h - a.H - a.Hk : h - a.H);
-        const void* src = is_q ? a.q : (is_v ? a.v : a.k);
-        const uint64_t pitch = is_q ? a.q_pitch : (is_v ? a.v_pitch : a.k_pitch);
-        const uint64_t col = (uint64_t)hk * a.Dh + c * 8;
-        Vec8 raw[U];
+// Sum over a group's lanes.
+template <int LPH>
+__device__ __forceinline__ float group_sum(float v) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const uint32_t rl = gr + u * a.GR;
-            raw[u] = load8<T>(src, (row0 + rl) * pitch + col, on && rl < nrows);
-        }
-        const void* gain = is_q ? a.gq : a.gk;
-        float w[8];
-        load_gain<T>(gain, c, lane_on, w);
-        if (first) {
-            fill_angles(a, s_cs, row0, nrows);
-            __syncthreads();
-            first = false;
-        }
-        void* dst = is_q ? a.qo : (is_v ? a.vo : a.ko);
-        const uint64_t opitch = is_q ? a.qo_pitch : a.ko_pitch;
+    for (int o = LPH / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o, LPH);
+    return v;
+}
+
+// The lane's sixteen gains, or ones.
+template <typename T, int LPH>
+__device__ __forceinline__ void load_gain(const void* gain, uint32_t c, uint32_t Dh, float (&w)[2][8]) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const uint32_t rl = gr + u * a.GR, row = row0 + rl;
-            float f[8], ss[1] = {0.0f};
-            unpack8<T>(raw[u], f);
+    for (int v = 0; v < 2; ++v) {
+        const uint32_t n = c + v * LPH;
+        if (gain && n * 8 < Dh) {
+            unpack8<T>(ld_vec8(reinterpret_cast<const T*>(gain) + n * 8), w[v]);
+        } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) ss[0] += f[e] * f[e];
-            group_sums<LPH, 1>(ss);
-            const float r = rsqrtf(ss[0] * a.inv_dh + a.eps);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] *= r * w[e];
-            rotate8<LPH>(a, s_cs + min(rl, nrows - 1) * half, c, 1.0f, f);
-            bool st = on && rl < nrows;
-            uint64_t at = row;
-            if (a.cache && !is_q && st) {
-                const int32_t pos = position(a, row);
-                st = pos >= 0 && (uint32_t)pos < a.cache_len;  // outside the cache: not stored
-                at = (uint64_t)(row / a.S) * a.cache_len + (uint32_t)pos;
-            }
-            if (st) st_vec8(reinterpret_cast<T*>(dst) + at * opitch + col, is_v ? raw[u] : pack8<T>(f));
+            for (int e = 0; e < 8; ++e) w[v][e] = 1.0f;
         }
     }
 }
 
-// Block b walks row tiles b, b + gridDim.x, ...: each lane adds its columns'
-// gain gradients over all heads it meets, the block adds its groups in order
-// and stores one partial row, and qk_gain_kernel adds the partials in order,
-// so the sums do not depend on timing.
-template <typename T, int LPH, int U>
-__global__ void __launch_bounds__(kThreads, kBwdBlocks) qk_backward_kernel(const __grid_constant__ QkArgs a) {
-    extern __shared__ __align__(16) float2 s_cs[];  // [GR U][angle_pitch]; then the groups' sums [G][2][Dh]
-    constexpr uint32_t G = kThreads / LPH;
+// Asynchronous 16-byte copies to the thread's own slots in shared memory: the
+// loads in flight need no registers, and no thread reads another's slot.
+__device__ __forceinline__ void cp16(Vec8* dst, const void* src, bool ok) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                     static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+                 "l"(src), "r"(ok ? 16 : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// A block walks row tiles b, b + gridDim.x, ... in rounds of one head of U
+// rows a group; the copies of the next LA rounds, running on from one tile
+// into the next, are in flight while one is worked on.
+template <typename T, int LPH, int U, int LA>
+__global__ void __launch_bounds__(kThreads, U == 1 ? 4 : kFwdBlocks)
+    qk_forward_kernel(const __grid_constant__ QkArgs a) {
+    extern __shared__ __align__(16) uint8_t s_raw[];
+    Vec8* slot = reinterpret_cast<Vec8*>(s_raw) + threadIdx.x;                     // [LA U][2][kThreads]
+    float2* s_cs = reinterpret_cast<float2*>(s_raw + 2 * LA * U * kThreads * 16);  // [GR U][angle_pitch]
     const uint32_t c = threadIdx.x % LPH, g = threadIdx.x / LPH;
-    const uint32_t gh = g % a.GH, gr = g / a.GH, half = angle_pitch(a.rot);
-    const uint32_t total = a.H + a.Hk, R = a.GR * U;
-    const bool lane_on = c * 8 < a.Dh;
-    float accq[8] = {}, acck[8] = {};
-    if (a.partial) pdl_trigger();  // qk_gain_kernel, which waits for this one to end
+    const uint32_t gh = g % a.GH, gr = g / a.GH, pitch = angle_pitch(a.rot);
+    const uint32_t total = a.H + a.Hk + (a.v ? a.Hk : 0);
+    const uint32_t h_begin = blockIdx.y * a.heads_per_block, h_end = min(total, h_begin + a.heads_per_block);
+    const uint32_t rounds = (h_end - h_begin + a.GH - 1) / a.GH, R = a.GR * U;
+    const bool lane0 = c * 8 < a.Dh, lane1 = (c + LPH) * 8 < a.Dh;
+    uint32_t next_row0 = blockIdx.x * R, next_round = 0, next_slot = 0;  // what is requested next
+    auto request = [&]() {
+        if (next_row0 < a.rows) {
+            const uint32_t h = h_begin + next_round * a.GH + gh;
+            const bool is_q = h < a.H, is_v = h >= a.H + a.Hk;
+            const uint32_t hk = is_q ? h : (is_v ? h - a.H - a.Hk : h - a.H);
+            const T* src = reinterpret_cast<const T*>(is_q ? a.q : (is_v ? a.v : a.k)) + (uint64_t)hk * a.Dh + c * 8;
+            const uint64_t step = is_q ? a.q_pitch : (is_v ? a.v_pitch : a.k_pitch);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const uint32_t row = next_row0 + gr + u * a.GR;
+                const bool ok = h < h_end && row < a.rows;
+                const T* p = ok ? src + row * step : reinterpret_cast<const T*>(a.q);
+                Vec8* s = slot + (next_slot * U + u) * 2 * kThreads;
+                cp16(s, p, ok && lane0);
+                cp16(s + kThreads, ok && lane1 ? p + LPH * 8 : p, ok && lane1);
+            }
+            if (++next_round == rounds) next_round = 0, next_row0 += gridDim.x * R;
+            if (++next_slot == LA) next_slot = 0;
+        }
+        cp_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < LA; ++i) request();
+    uint32_t cur = 0;
     for (uint32_t row0 = blockIdx.x * R; row0 < a.rows; row0 += gridDim.x * R) {
         const uint32_t nrows = min(R, a.rows - row0);
-        bool first = true;
-        for (uint32_t h0 = 0; h0 < total; h0 += a.GH) {
-            const uint32_t h = h0 + gh;
-            const bool on = h < total && lane_on, is_q = h < a.H;
-            const uint64_t col = (uint64_t)(is_q ? h : h - a.H) * a.Dh + c * 8;
-            Vec8 rx[U], rt[U];
+        if (row0 != blockIdx.x * R) __syncthreads();  // the previous tile's angles have been read
+        fill_angles(a, s_cs, row0, nrows);
+        __syncthreads();
+        for (uint32_t round = 0; round < rounds; ++round) {
+            const uint32_t h = h_begin + round * a.GH + gh;
+            const bool on = h < h_end, is_q = h < a.H, is_v = h >= a.H + a.Hk;
+            const uint32_t hk = is_q ? h : (is_v ? h - a.H - a.Hk : h - a.H);
+            float w[2][8];
+            load_gain<T, LPH>(is_q ? a.gq : a.gk, c, a.Dh, w);
+            T* dst = reinterpret_cast<T*>(is_q ? a.qo : (is_v ? a.vo : a.ko)) + (uint64_t)hk * a.Dh + c * 8;
+            const uint64_t opitch = is_q ? a.qo_pitch : a.ko_pitch;
+            cp_wait<LA - 1>();
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const uint32_t rl = gr + u * a.GR, row = row0 + rl;
-                const bool ld = on && rl < nrows;
-                rx[u] = load8<T>(is_q ? a.q : a.k, row * (is_q ? a.q_pitch : a.k_pitch) + col, ld);
-                rt[u] = load8<T>(is_q ? a.dqo : a.dko, row * (is_q ? a.dqo_pitch : a.dko_pitch) + col, ld);
-            }
-            const void* gain = is_q ? a.gq : a.gk;
-            float w[8];
-            load_gain<T>(gain, c, lane_on, w);
-            if (first) {
-                __syncthreads();  // the previous tile's angles have been read
-                fill_angles(a, s_cs, row0, nrows);
-                __syncthreads();
-                first = false;
-            }
-            float x[U][8], t[U][8], ss[U], m[U], acc[8] = {};
+                const Vec8* s = slot + (cur * U + u) * 2 * kThreads;
+                const Vec8 raw0 = ld_shared_vec8(s), raw1 = ld_shared_vec8(s + kThreads);
+                float f[2][8], ss = 0.0f;
+                unpack8<T>(raw0, f[0]);
+                unpack8<T>(raw1, f[1]);
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                unpack8<T>(rx[u], x[u]);
-                unpack8<T>(rt[u], t[u]);
-                ss[u] = 0.0f;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) ss[u] += x[u][e] * x[u][e];
-            }
-            group_sums<LPH, U>(ss);
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                rotate8<LPH>(a, s_cs + min(gr + u * a.GR, nrows - 1) * half, c, -1.0f, t[u]);
-                ss[u] = rsqrtf(ss[u] * a.inv_dh + a.eps);
-                m[u] = 0.0f;
+                for (int e = 0; e < 8; ++e) ss += f[0][e] * f[0][e] + f[1][e] * f[1][e];
+                const float r = rsqrtf(group_sum<LPH>(ss) * a.inv_dh + a.eps);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    x[u][e] *= ss[u];  // n
-                    acc[e] += t[u][e] * x[u][e];
-                    t[u][e] *= w[e];  // dn
-                    m[u] += t[u][e] * x[u][e];
+                    f[0][e] *= r * w[0][e];
+                    f[1][e] *= r * w[1][e];
                 }
+                rotate<LPH>(a, s_cs + min(rl, nrows - 1) * pitch, c, 1.0f, f);
+                bool st = on && rl < nrows;
+                uint64_t at = row;
+                if (a.cache && !is_q && st) {
+                    const int32_t pos = position(a, row);
+                    st = pos >= 0 && (uint32_t)pos < a.cache_len;  // outside the cache: not stored
+                    at = (uint64_t)(row / a.S) * a.cache_len + (uint32_t)pos;
+                }
+                T* p = dst + at * opitch;
+                if (st && lane0) st_vec8(p, is_v ? raw0 : pack8<T>(f[0]));
+                if (st && lane1) st_vec8(p + LPH * 8, is_v ? raw1 : pack8<T>(f[1]));
             }
-            group_sums<LPH, U>(m);
-            T* dst = reinterpret_cast<T*>(is_q ? a.qo : a.ko) + col;
+            if (++cur == LA) cur = 0;
+            request();
+        }
+    }
+}
+
+// The same walk.  Each lane adds its columns' gain gradients over all heads it
+// meets, the block adds its groups in order and stores one partial row, and
+// qk_gain_kernel adds the partials in order, so the sums do not depend on
+// timing.
+template <typename T, int LPH, int U, int LA>
+__global__ void __launch_bounds__(kThreads, kBwdBlocks) qk_backward_kernel(const __grid_constant__ QkArgs a) {
+    extern __shared__ __align__(16) uint8_t s_raw[];
+    Vec8* slot = reinterpret_cast<Vec8*>(s_raw) + threadIdx.x;  // [LA U][x, dy][2][kThreads]
+    // [GR U][angle_pitch]; then, over all of it, the groups' sums [G][2][Dh]
+    float2* s_cs = reinterpret_cast<float2*>(s_raw + 4 * LA * U * kThreads * 16);
+    constexpr uint32_t G = kThreads / LPH;
+    const uint32_t c = threadIdx.x % LPH, g = threadIdx.x / LPH;
+    const uint32_t gh = g % a.GH, gr = g / a.GH, pitch = angle_pitch(a.rot);
+    const uint32_t total = a.H + a.Hk, R = a.GR * U, rounds = (total + a.GH - 1) / a.GH;
+    const bool lane0 = c * 8 < a.Dh, lane1 = (c + LPH) * 8 < a.Dh;
+    float accq[2][8] = {}, acck[2][8] = {};
+    if (a.partial) pdl_trigger();  // qk_gain_kernel, which waits for this one to end
+    uint32_t next_row0 = blockIdx.x * R, next_round = 0, next_slot = 0;  // what is requested next
+    auto request = [&]() {
+        if (next_row0 < a.rows) {
+            const uint32_t h = next_round * a.GH + gh;
+            const bool is_q = h < a.H;
+            const uint64_t col = (uint64_t)(is_q ? h : h - a.H) * a.Dh + c * 8;
+            const T* x = reinterpret_cast<const T*>(is_q ? a.q : a.k) + col;
+            const T* t = reinterpret_cast<const T*>(is_q ? a.dqo : a.dko) + col;
+            const uint64_t xs = is_q ? a.q_pitch : a.k_pitch, ts = is_q ? a.dqo_pitch : a.dko_pitch;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const uint32_t row = next_row0 + gr + u * a.GR;
+                const bool ok = h < total && row < a.rows;
+                const T* px = ok ? x + row * xs : reinterpret_cast<const T*>(a.q);
+                const T* pt = ok ? t + row * ts : reinterpret_cast<const T*>(a.q);
+                Vec8* s = slot + (next_slot * U + u) * 4 * kThreads;
+                cp16(s, px, ok && lane0);
+                cp16(s + kThreads, ok && lane1 ? px + LPH * 8 : px, ok && lane1);
+                cp16(s + 2 * kThreads, pt, ok && lane0);
+                cp16(s + 3 * kThreads, ok && lane1 ? pt + LPH * 8 : pt, ok && lane1);
+            }
+            if (++next_round == rounds) next_round = 0, next_row0 += gridDim.x * R;
+            if (++next_slot == LA) next_slot = 0;
+        }
+        cp_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < LA; ++i) request();
+    uint32_t cur = 0;
+    for (uint32_t row0 = blockIdx.x * R; row0 < a.rows; row0 += gridDim.x * R) {
+        const uint32_t nrows = min(R, a.rows - row0);
+        if (row0 != blockIdx.x * R) __syncthreads();  // the previous tile's angles have been read
+        fill_angles(a, s_cs, row0, nrows);
+        __syncthreads();
+        for (uint32_t round = 0; round < rounds; ++round) {
+            const uint32_t h = round * a.GH + gh;
+            const bool on = h < total, is_q = h < a.H;
+            float w[2][8], acc[2][8] = {};
+            load_gain<T, LPH>(is_q ? a.gq : a.gk, c, a.Dh, w);
+            T* dst = reinterpret_cast<T*>(is_q ? a.qo : a.ko) + (uint64_t)(is_q ? h : h - a.H) * a.Dh + c * 8;
             const uint64_t opitch = is_q ? a.qo_pitch : a.ko_pitch;
+            cp_wait<LA - 1>();
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const uint32_t rl = gr + u * a.GR;
-                m[u] *= a.inv_dh;
+                const Vec8* s = slot + (cur * U + u) * 4 * kThreads;
+                float x[2][8], t[2][8], ss = 0.0f, m = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) t[u][e] = ss[u] * (t[u][e] - x[u][e] * m[u]);
-                if (on && rl < nrows) st_vec8(dst + (row0 + rl) * opitch, pack8<T>(t[u]));
+                for (int v = 0; v < 2; ++v) {
+                    unpack8<T>(ld_shared_vec8(s + v * kThreads), x[v]);
+                    unpack8<T>(ld_shared_vec8(s + (2 + v) * kThreads), t[v]);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) ss += x[v][e] * x[v][e];
+                }
+                const float r = rsqrtf(group_sum<LPH>(ss) * a.inv_dh + a.eps);
+                rotate<LPH>(a, s_cs + min(rl, nrows - 1) * pitch, c, -1.0f, t);
+#pragma unroll
+                for (int v = 0; v < 2; ++v)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        x[v][e] *= r;  // n
+                        acc[v][e] += t[v][e] * x[v][e];
+                        t[v][e] *= w[v][e];  // dn
+                        m += t[v][e] * x[v][e];
+                    }
+                m = group_sum<LPH>(m) * a.inv_dh;
+#pragma unroll
+                for (int v = 0; v < 2; ++v)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) t[v][e] = r * (t[v][e] - x[v][e] * m);
+                T* p = dst + (row0 + rl) * opitch;
+                if (on && rl < nrows && lane0) st_vec8(p, pack8<T>(t[0]));
+                if (on && rl < nrows && lane1) st_vec8(p + LPH * 8, pack8<T>(t[1]));
             }
+            if (++cur == LA) cur = 0;
+            request();
             if (!a.partial) continue;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if (is_q) accq[e] += acc[e];
-                else acck[e] += acc[e];
-            }
+            for (int v = 0; v < 2; ++v)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if (is_q) accq[v][e] += acc[v][e];
+                    else acck[v][e] += acc[v][e];
+                }
         }
     }
     if (!a.partial) return;
-    float* sums = reinterpret_cast<float*>(s_cs);
+    cp_wait<0>();
+    float* sums = reinterpret_cast<float*>(s_raw);
     __syncthreads();
-    if (lane_on) {
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+        if (v ? !lane1 : !lane0) continue;
+        float* p = sums + g * 2 * a.Dh + (c + v * LPH) * 8;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            sums[(g * 2 + 0) * a.Dh + c * 8 + e] = accq[e];
-            sums[(g * 2 + 1) * a.Dh + c * 8 + e] = acck[e];
+            p[e] = accq[v][e];
+            p[a.Dh + e] = acck[v][e];
         }
     }
     __syncthreads();
@@ -330,16 +431,16 @@ __global__ void __launch_bounds__(1024) qk_gain_kernel(const float* partial, uin
     *dst = Elem<T>::from_f(acc ? Elem<T>::to_f(*dst) + t : t);
 }
 
-uint32_t lanes_per_head(uint32_t Dh) { return Dh <= 32 ? 4 : Dh <= 64 ? 8 : Dh <= 128 ? 16 : 32; }
+uint32_t lanes_per_head(uint32_t Dh) { return Dh <= 32 ? 2 : Dh <= 64 ? 4 : Dh <= 128 ? 8 : 16; }
 
 // Calls f with the lanes-per-head constant of head size Dh.
 template <class F>
 int with_lph(uint32_t Dh, F&& f) {
     switch (lanes_per_head(Dh)) {
+        case 2: return f(std::integral_constant<int, 2>());
         case 4: return f(std::integral_constant<int, 4>());
         case 8: return f(std::integral_constant<int, 8>());
-        case 16: return f(std::integral_constant<int, 16>());
-        default: return f(std::integral_constant<int, 32>());
+        default: return f(std::integral_constant<int, 16>());
     }
 }
 
@@ -454,11 +555,16 @@ extern "C" int evkcu_qk_norm_rope(const evkcu_qk_norm_rope_desc* d, const void* 
     a.heads_per_block = large ? total : a.GH;
     return EVKCU_DISPATCH_DTYPE(dtype, T, [&] {
         return with_lph(a.Dh, [&](auto lph) {
-            const uint32_t R = a.GR * (large ? kFwdRows : 1);
-            const dim3 grid((a.rows + R - 1) / R, large ? 1 : (uint32_t)rounds);
-            const size_t smem = R * angle_pitch(a.rot) * sizeof(float2);  // at most 32 KB
-            if (large) qk_forward_kernel<T, lph.value, kFwdRows><<<grid, kThreads, smem, as_stream(stream)>>>(a);
-            else qk_forward_kernel<T, lph.value, 1><<<grid, kThreads, smem, as_stream(stream)>>>(a);
+            const uint32_t R = a.GR * (large ? kFwdRows : 1), tiles = (a.rows + R - 1) / R;
+            const size_t smem = 2 * (large ? kFwdRows * kFwdAhead : 1) * kThreads * 16 +
+                                R * angle_pitch(a.rot) * sizeof(float2);
+            auto kern = large ? qk_forward_kernel<T, lph.value, kFwdRows, kFwdAhead>
+                              : qk_forward_kernel<T, lph.value, 1, 1>;
+            static std::atomic<uint64_t> done[2];
+            EVKCU_TRY(allow_smem(kern, kMaxSmem, done[large]));
+            const dim3 grid(large ? std::min(tiles, kFwdBlocks * (uint32_t)ds->sm_count) : tiles,
+                            large ? 1 : (uint32_t)rounds);
+            kern<<<grid, kThreads, smem, as_stream(stream)>>>(a);
             return after_launch("evkcu_qk_norm_rope");
         });
     });
@@ -521,9 +627,12 @@ extern "C" int evkcu_qk_norm_rope_backward(const evkcu_qk_norm_rope_desc* d, con
             constexpr uint32_t U = kBwdRows;
             const uint32_t R = a.GR * U, tiles = (a.rows + R - 1) / R;
             const uint32_t grid = std::min({tiles, kMaxPartials, kBwdBlocks * (uint32_t)ds->sm_count});  // resident at once
-            const size_t smem = std::max<size_t>(R * angle_pitch(a.rot) * sizeof(float2),
+            const size_t smem = std::max<size_t>(4 * U * kBwdAhead * kThreads * 16 + R * angle_pitch(a.rot) * sizeof(float2),
                                                  gains ? (size_t)(kThreads / lph.value) * 2 * a.Dh * sizeof(float) : 0);
-            qk_backward_kernel<T, lph.value, U><<<grid, kThreads, smem, st>>>(a);
+            auto kern = qk_backward_kernel<T, lph.value, U, kBwdAhead>;
+            static std::atomic<uint64_t> done{0};
+            EVKCU_TRY(allow_smem(kern, kMaxSmem, done));
+            kern<<<grid, kThreads, smem, st>>>(a);
             EVKCU_TRY(after_launch("evkcu_qk_norm_rope_backward"));
             if (!gains) return (int)EVKCU_OK;
             return launch_pdl("evkcu_qk_norm_rope_backward(gains)", qk_gain_kernel<T>, dim3((2 * a.Dh + 31) / 32),
