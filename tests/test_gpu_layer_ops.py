@@ -322,6 +322,24 @@ def test_gated_ffn_backward(rows, D, F, act, dt, nk, acc):
         check(got.t, ref, rounded(ref, e, dt), name)
 
 
+@pytest.mark.parametrize("rows", [9, 200, 2100])
+def test_gated_ffn_alone_and_gradient_in_place(rows):
+    """y = None stops at hidden (a gated linear unit); dpre may be pre."""
+    dt, g, D, F = torch.bfloat16, gen(rows), 264, 1368
+    x, wi, wo = rnd(g, dt, rows, D), rnd(g, dt, D, 2 * F, std=D ** -0.5), rnd(g, dt, F, D, std=F ** -0.5)
+    h, z = Guarded(dt, rows, F), Guarded(dt, rows, 2 * F)
+    assert evk.gated_ffn(x, wi, None, None, h.t, pre=z.t) is h.t
+    h.check(), z.check()
+    zr, tz, hr, th, _, _ = ffn_ref(x, wi, wo, None, "silu", dt)
+    check(h.t, hr, th, "hidden")
+    check(z.t, zr, tz, "pre")
+    dy, pre = rnd(g, dt, rows, D), z.t.clone()
+    dx, dz, d2 = torch.empty_like(x), torch.empty_like(pre), torch.empty_like(x)
+    evk.gated_ffn_backward(x, wi, wo, pre, dy, dz, None, dx=dx)
+    evk.gated_ffn_backward(x, wi, wo, pre, dy, pre, None, dx=d2)
+    assert torch.equal(pre, dz) and torch.equal(dx, d2)
+
+
 @pytest.mark.parametrize("act", ["gelu", "silu"])
 def test_gradients_against_differences(act):
     """The kernels' gradients of L = sum(y * dy) against central differences of
@@ -398,6 +416,36 @@ def test_no_rows(dt):
     evk.qk_norm_rope(q, q, q, q, 2)
     evk.qk_norm_rope_backward(q, None, q, None, q, None, 2, dgain_q=dg)
     assert not bool(dg.any())
+
+
+def test_more_than_2_31_elements():
+    """Offsets past 32 bits: outputs, saved tensors and a cache of 2.2e9
+    elements, looked at near both ends."""
+    dt, g = torch.bfloat16, gen(31)
+    rows, K, N = 270001, 8, 8192
+    x, w = rnd(g, dt, rows, K), rnd(g, dt, K, N)
+    y = torch.empty(rows, N, dtype=dt, device="cuda")
+    evk.linear(x, w, y, residual=None, act=evk.ACT_SILU)
+    dx, dz = torch.empty_like(x), torch.empty_like(y)
+    evk.linear_backward(x, w, y, dx=dx, act=evk.ACT_SILU, pre=y, dpre=dz)
+    for at in (slice(0, 300), slice(rows - 300, rows)):
+        _, _, yr, tol = lin_ref(x[at], w, None, None, "silu", dt)
+        check(y[at], yr, tol, "y")
+        dzr, ez, (dxr, edx), _, _ = back_ref(x[at], w, y[at], y[at], "silu", dt)
+        check(dz[at], dzr, ez, "dpre")
+        check(dx[at], dxr, rounded(dxr, edx, dt), "dx")
+    del y, dz
+    cache_len, heads, dh = 1100000, 16, 128
+    kc, vc = (torch.zeros(1, cache_len, heads * dh, dtype=dt, device="cuda") for _ in range(2))
+    k, v = rnd(g, dt, 1, 3, heads * dh), rnd(g, dt, 1, 3, heads * dh)
+    pos = torch.tensor([[0, cache_len - 1, cache_len // 2]], dtype=torch.int32, device="cuda")
+    evk.qk_norm_rope(k, k, torch.empty_like(k), kc, heads, v=v, v_out=vc, cache=True, positions=pos)
+    kr, n, _, wt, _, spread = qk_ref(k, heads, None, pos, 0, False, 10000.0, 1e-5)
+    tol = rounded(kr, 2 * qk_unit(dh) * spread(n * wt), dt)
+    for t in range(3):
+        check(kc[0, pos[0, t]].reshape(heads, dh), kr[0, t], tol[0, t], "cache row")
+        assert torch.equal(vc[0, pos[0, t]], v[0, t])
+    assert int(torch.count_nonzero(vc.view(torch.int16)[0].any(-1))) == 3
 
 
 # ------------------------------------------------------------- qk_norm_rope --
