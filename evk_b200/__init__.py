@@ -132,12 +132,25 @@ def _check(op: str, status: int) -> None:
         raise EvkcuError(op, status, lib().evkcu_last_error().decode())
 
 
-def _dtype_code(t) -> int:
-    import torch
+_torch = None
 
-    if t.dtype == torch.float16:
+
+def _get_torch():
+    """torch, imported on first use (an import statement in every call costs
+    more than a look at a global)."""
+    global _torch
+    if _torch is None:
+        import torch
+
+        _torch = torch
+    return _torch
+
+
+def _dtype_code(t) -> int:
+    torch = _torch or _get_torch()
+    if t.dtype is torch.float16:
         return F16
-    if t.dtype == torch.bfloat16:
+    if t.dtype is torch.bfloat16:
         return BF16
     raise TypeError(f"unsupported dtype {t.dtype}: evk tensors are 2-byte fp16 (or bf16)")
 
@@ -153,10 +166,9 @@ def _ptr(t) -> int:
 
 
 def _stream(stream) -> int:
-    import torch
-
     if stream is None:
         # the raw handle, without building a Stream object (3 us a call)
+        torch = _torch or _get_torch()
         return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
     return getattr(stream, "cuda_stream", stream)
 
@@ -457,23 +469,38 @@ SIGNATURES.update({
 _RET["evkcu_qk_norm_rope_workspace"] = _u64
 
 
-def _same(op, like, *want):
+def _same(op, like, want):
     """Checks (name, tensor or None, shape) triples against `like`'s dtype and
     device, which has to be the current one."""
-    import torch
-
     dt, dev = like.dtype, like.get_device()
-    for i in range(0, len(want), 3):
-        t = want[i + 1]
+    for name, t, shape in want:
         if t is None:
             continue
-        if t.dtype != dt or t.get_device() != dev:
-            raise EvkcuError(op, 7, f"{want[i]} is {t.dtype} on {t.device}, expected {dt} on {like.device}")
-        if t.shape != want[i + 2]:
-            raise EvkcuError(op, 1, f"{want[i]} is {tuple(t.shape)}, expected {tuple(want[i + 2])}")
-    if dev >= 0 and dev != torch.cuda.current_device():
+        if t.dtype is not dt or t.get_device() != dev:
+            raise EvkcuError(op, 7, f"{name} is {t.dtype} on {t.device}, expected {dt} on {like.device}")
+        if t.shape != shape:
+            raise EvkcuError(op, 1, f"{name} is {tuple(t.shape)}, expected {tuple(shape)}")
+    if dev < 0:
+        raise ValueError("evk_b200 ops take CUDA tensors")
+    torch = _torch or _get_torch()
+    if dev != torch.cuda.current_device():
         raise EvkcuError(op, 7, f"tensors are on cuda:{dev}, the current device is "
                                 f"cuda:{torch.cuda.current_device()}")
+
+
+def _same_ptrs(op, like, want):
+    """_same, and the pointers of the tensors (None for none), which have to be
+    contiguous."""
+    _same(op, like, want)
+    out = []
+    for name, t, _ in want:
+        if t is None:
+            out.append(None)
+        elif t.is_contiguous():
+            out.append(t.data_ptr())
+        else:
+            raise ValueError(f"evk_b200 ops take contiguous (row-major) tensors: {name}")
+    return out
 
 
 def linear(x, w, y, bias=None, residual=None, act=ACT_NONE, pre=None, transpose_w=False, stream=None):
@@ -485,11 +512,11 @@ def linear(x, w, y, bias=None, residual=None, act=ACT_NONE, pre=None, transpose_
     *lead, K = x.shape
     N = y.shape[-1]
     out = (*lead, N)
-    _same("linear", x, "w", w, (N, K) if transpose_w else (K, N), "y", y, out, "bias", bias, (N,), "residual",
-          residual, out, "pre", pre, out)
+    p = _same_ptrs("linear", x, (("x", x, x.shape), ("w", w, (N, K) if transpose_w else (K, N)), ("bias", bias, (N,)),
+                                 ("residual", residual, out), ("y", y, out), ("pre", pre, out)))
     _check("evkcu_linear", lib().evkcu_linear(
-        _ptr(x), _ptr(w), _ptr(bias), _ptr(residual), _ptr(y), _ptr(pre), x.numel() // K if K else 0, K, N, act,
-        MM_TRANSPOSE_B if transpose_w else 0, _dtype_code(x), _stream(stream)))
+        *p, x.numel() // K if K else 0, K, N, act, MM_TRANSPOSE_B if transpose_w else 0, _dtype_code(x),
+        _stream(stream)))
     return y
 
 
@@ -502,12 +529,12 @@ def linear_backward(x, w, dy, dx=None, dw=None, dbias=None, act=ACT_NONE, pre=No
     K, N = x.shape[-1], dy.shape[-1]
     out = (*x.shape[:-1], N)
     wshape = (N, K) if transpose_w else (K, N)
-    _same("linear_backward", x, "w", w, wshape, "dy", dy, out, "dx", dx, x.shape, "dw", dw, wshape, "dbias", dbias,
-          (N,), "pre", pre, out, "dpre", dpre, out)
+    p = _same_ptrs("linear_backward", x, (("x", x, x.shape), ("w", w, wshape), ("pre", pre, out), ("dy", dy, out),
+                                          ("dpre", dpre, out), ("dx", dx, x.shape), ("dw", dw, wshape),
+                                          ("dbias", dbias, (N,))))
     flags = (MM_TRANSPOSE_B if transpose_w else 0) | (MM_ACC_C if acc else 0)
     _check("evkcu_linear_backward", lib().evkcu_linear_backward(
-        _ptr(x), _ptr(w), _ptr(pre), _ptr(dy), _ptr(dpre), _ptr(dx), _ptr(dw), _ptr(dbias),
-        x.numel() // K if K else 0, K, N, act, flags, _dtype_code(x), _stream(stream)))
+        *p, x.numel() // K if K else 0, K, N, act, flags, _dtype_code(x), _stream(stream)))
     return dx, dw, dbias
 
 
@@ -520,12 +547,12 @@ def gated_ffn(x, w_in, w_out, y, hidden, act=ACT_SILU, residual=None, pre=None, 
     gated_ffn_backward.  y = None (then w_out may be None) stops at hidden."""
     D, F = x.shape[-1], hidden.shape[-1]
     lead = x.shape[:-1]
-    _same("gated_ffn", x, "w_in", w_in, (2 * F, D) if transpose_w else (D, 2 * F), "w_out", w_out,
-          (D, F) if transpose_w else (F, D), "y", y, x.shape, "hidden", hidden, (*lead, F), "residual", residual,
-          x.shape, "pre", pre, (*lead, 2 * F))
+    p = _same_ptrs("gated_ffn", x, (("x", x, x.shape), ("w_in", w_in, (2 * F, D) if transpose_w else (D, 2 * F)),
+                                    ("w_out", w_out, (D, F) if transpose_w else (F, D)),
+                                    ("residual", residual, x.shape), ("y", y, x.shape), ("hidden", hidden, (*lead, F)),
+                                    ("pre", pre, (*lead, 2 * F))))
     _check("evkcu_gated_ffn", lib().evkcu_gated_ffn(
-        _ptr(x), _ptr(w_in), _ptr(w_out), _ptr(residual), _ptr(y), _ptr(hidden), _ptr(pre),
-        x.numel() // D if D else 0, D, F, act, MM_TRANSPOSE_B if transpose_w else 0, _dtype_code(x),
+        *p, x.numel() // D if D else 0, D, F, act, MM_TRANSPOSE_B if transpose_w else 0, _dtype_code(x),
         _stream(stream)))
     return y if y is not None else hidden
 
@@ -539,21 +566,19 @@ def gated_ffn_backward(x, w_in, w_out, pre, dy, dpre, hidden, dx=None, dw_in=Non
     D, F = x.shape[-1], pre.shape[-1] // 2
     lead = x.shape[:-1]
     si, so = ((2 * F, D), (D, F)) if transpose_w else ((D, 2 * F), (F, D))
-    _same("gated_ffn_backward", x, "w_in", w_in, si, "w_out", w_out, so, "pre", pre, (*lead, 2 * F), "dy", dy,
-          x.shape, "dpre", dpre, (*lead, 2 * F), "hidden", hidden, (*lead, F), "dx", dx, x.shape, "dw_in", dw_in, si,
-          "dw_out", dw_out, so)
+    p = _same_ptrs("gated_ffn_backward", x, (("x", x, x.shape), ("w_in", w_in, si), ("w_out", w_out, so),
+                                             ("pre", pre, (*lead, 2 * F)), ("dy", dy, x.shape),
+                                             ("dpre", dpre, (*lead, 2 * F)), ("hidden", hidden, (*lead, F)),
+                                             ("dx", dx, x.shape), ("dw_in", dw_in, si), ("dw_out", dw_out, so)))
     flags = (MM_TRANSPOSE_B if transpose_w else 0) | (MM_ACC_C if acc else 0)
     _check("evkcu_gated_ffn_backward", lib().evkcu_gated_ffn_backward(
-        _ptr(x), _ptr(w_in), _ptr(w_out), _ptr(pre), _ptr(dy), _ptr(dpre), _ptr(hidden), _ptr(dx), _ptr(dw_in),
-        _ptr(dw_out), x.numel() // D if D else 0, D, F, act, flags, _dtype_code(x), _stream(stream)))
+        *p, x.numel() // D if D else 0, D, F, act, flags, _dtype_code(x), _stream(stream)))
     return dx, dw_in, dw_out
 
 
 def _rows(op, name, t, B, S):
     """(pointer, row pitch) of a (B, S, cols) tensor whose rows are evenly
     spaced (a slice of the last dimension of a contiguous tensor is)."""
-    if not t.is_cuda:
-        raise ValueError("evk_b200 ops take CUDA tensors")
     sb, st, sc = t.stride()
     if (sc != 1 and t.shape[2] > 1) or (B > 1 and S > 1 and sb != S * st):
         raise EvkcuError(op, 1, f"{name}: strides {t.stride()} are not evenly spaced rows")
@@ -573,9 +598,8 @@ def _qk_shape(op, q, k, heads, positions, rot_dim, pos_offset):
         kc = k.shape[2]
     pos = None
     if positions is not None:
-        import torch
-
-        if positions.dtype != torch.int32 or positions.numel() != B * S or positions.get_device() != q.get_device():
+        torch = _torch or _get_torch()
+        if positions.dtype is not torch.int32 or positions.numel() != B * S or positions.get_device() != q.get_device():
             raise EvkcuError(op, 1, f"positions must be {B * S} int32 values on {q.device}")
         pos = _ptr(positions)
     if not 0 <= rot_dim <= 0xFFFFFFFF or not 0 <= pos_offset <= 0xFFFFFFFF:
@@ -606,8 +630,8 @@ def qk_norm_rope(q, k, q_out, k_out, heads: int, gain_q=None, gain_k=None, v=Non
         cache_len = k_out.shape[1]
     ks = (B, S, kc)
     os = (B, cache_len, kc) if cache else ks
-    _same(op, q, "q_out", q_out, q.shape, "gain_q", gain_q, (dh,), "gain_k", gain_k, (dh,), "k", k, ks, "k_out",
-          k_out if k is not None else None, os, "v", v, ks, "v_out", v_out, os)
+    _same(op, q, (("q_out", q_out, q.shape), ("gain_q", gain_q, (dh,)), ("gain_k", gain_k, (dh,)), ("k", k, ks),
+                  ("k_out", k_out if k is not None else None, os), ("v", v, ks), ("v_out", v_out, os)))
     qp, q_pitch = _rows(op, "q", q, B, S)
     qo, qo_pitch = _rows(op, "q_out", q_out, B, S)
     kp = ko = vp = vo = None
@@ -650,8 +674,9 @@ def qk_norm_rope_backward(q, k, dq_out, dk_out, dq, dk, heads: int, gain_q=None,
     ks = (B, S, kc)
     if k is None:
         dk_out = dk = None
-    _same(op, q, "dq_out", dq_out, q.shape, "dq", dq, q.shape, "gain_q", gain_q, (dh,), "gain_k", gain_k, (dh,),
-          "dgain_q", dgain_q, (dh,), "dgain_k", dgain_k, (dh,), "k", k, ks, "dk_out", dk_out, ks, "dk", dk, ks)
+    _same(op, q, (("dq_out", dq_out, q.shape), ("dq", dq, q.shape), ("gain_q", gain_q, (dh,)),
+                  ("gain_k", gain_k, (dh,)), ("dgain_q", dgain_q, (dh,)), ("dgain_k", dgain_k, (dh,)), ("k", k, ks),
+                  ("dk_out", dk_out, ks), ("dk", dk, ks)))
     qp, q_pitch = _rows(op, "q", q, B, S)
     gq, gq_pitch = _rows(op, "dq_out", dq_out, B, S)
     dqp, dq_pitch = _rows(op, "dq", dq, B, S)

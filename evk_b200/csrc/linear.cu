@@ -317,13 +317,12 @@ constexpr uint32_t kMaxDim = 1u << 30;  // TMA coordinates are signed 32-bit
 
 int check_common(const char* op, uint32_t rows, uint32_t a, uint32_t b, int act, uint32_t flags, uint32_t allowed,
                  int dtype) {
-    const std::string o(op);
-    EVKCU_CHECK_ARG(dtype == EVKCU_F16 || dtype == EVKCU_BF16, EVKCU_BAD_ARG, o + ": unknown dtype");
-    EVKCU_CHECK_ARG(act >= EVKCU_ACT_NONE && act <= EVKCU_ACT_SILU, EVKCU_BAD_ARG, o + ": unknown activation");
-    EVKCU_CHECK_ARG((flags & ~allowed) == 0, EVKCU_BAD_ARG, o + ": unknown flag");
+    EVKCU_CHECK_ARG(dtype == EVKCU_F16 || dtype == EVKCU_BF16, EVKCU_BAD_ARG, std::string(op) + ": unknown dtype");
+    EVKCU_CHECK_ARG(act >= EVKCU_ACT_NONE && act <= EVKCU_ACT_SILU, EVKCU_BAD_ARG, std::string(op) + ": unknown activation");
+    EVKCU_CHECK_ARG((flags & ~allowed) == 0, EVKCU_BAD_ARG, std::string(op) + ": unknown flag");
     EVKCU_CHECK_ARG(a > 0 && b > 0 && a % 8 == 0 && b % 8 == 0, EVKCU_BAD_SHAPE,
-                    o + ": feature sizes must be positive multiples of 8");
-    EVKCU_CHECK_ARG(rows <= kMaxDim && a <= kMaxDim && b <= kMaxDim, EVKCU_BAD_SHAPE, o + ": size above 2^30");
+                    std::string(op) + ": feature sizes must be positive multiples of 8");
+    EVKCU_CHECK_ARG(rows <= kMaxDim && a <= kMaxDim && b <= kMaxDim, EVKCU_BAD_SHAPE, std::string(op) + ": size above 2^30");
     return EVKCU_OK;
 }
 

@@ -455,25 +455,24 @@ void set_groups(QkArgs& a, uint32_t total) {
 
 bool pitch_ok(uint64_t pitch, uint64_t cols) { return pitch >= cols && pitch % 8 == 0 && pitch <= (1ull << 40); }
 
-int check_desc(const char* name, const evkcu_qk_norm_rope_desc* d, uint32_t allowed, int dtype) {
-    const std::string op(name);
-    EVKCU_CHECK_ARG(d, EVKCU_BAD_ARG, op + ": descriptor is null");
-    EVKCU_CHECK_ARG(dtype == EVKCU_F16 || dtype == EVKCU_BF16, EVKCU_BAD_ARG, op + ": unknown dtype");
-    EVKCU_CHECK_ARG((d->flags & ~allowed) == 0, EVKCU_BAD_ARG, op + ": unknown flag");
+int check_desc(const char* op, const evkcu_qk_norm_rope_desc* d, uint32_t allowed, int dtype) {
+    EVKCU_CHECK_ARG(d, EVKCU_BAD_ARG, std::string(op) + ": descriptor is null");
+    EVKCU_CHECK_ARG(dtype == EVKCU_F16 || dtype == EVKCU_BF16, EVKCU_BAD_ARG, std::string(op) + ": unknown dtype");
+    EVKCU_CHECK_ARG((d->flags & ~allowed) == 0, EVKCU_BAD_ARG, std::string(op) + ": unknown flag");
     EVKCU_CHECK_ARG(d->head_dim >= 8 && d->head_dim <= 256 && d->head_dim % 8 == 0, EVKCU_BAD_SHAPE,
-                    op + ": head_dim must be a multiple of 8, 8 to 256");
+                    std::string(op) + ": head_dim must be a multiple of 8, 8 to 256");
     const uint32_t step = (d->flags & EVKCU_QK_HALF_SPLIT) ? 16 : 2;
     EVKCU_CHECK_ARG(d->rot_dim <= d->head_dim && (d->rot_dim ? d->rot_dim : d->head_dim) % step == 0, EVKCU_BAD_SHAPE,
-                    op + ": rot_dim must be at most head_dim and a multiple of 2 (of 16 for half-split pairs)");
+                    std::string(op) + ": rot_dim must be at most head_dim and a multiple of 2 (of 16 for half-split pairs)");
     EVKCU_CHECK_ARG(d->heads > 0 && d->heads <= 65535 && d->kv_heads <= 65535, EVKCU_BAD_SHAPE,
-                    op + ": heads must be 1 to 65535, kv_heads at most 65535");
-    EVKCU_CHECK_ARG((uint64_t)d->batch * d->seq_len <= (1ull << 30), EVKCU_BAD_SHAPE, op + ": more than 2^30 rows");
+                    std::string(op) + ": heads must be 1 to 65535, kv_heads at most 65535");
+    EVKCU_CHECK_ARG((uint64_t)d->batch * d->seq_len <= (1ull << 30), EVKCU_BAD_SHAPE, std::string(op) + ": more than 2^30 rows");
     EVKCU_CHECK_ARG(d->positions || (uint64_t)d->pos_offset + d->seq_len <= (1ull << 31), EVKCU_BAD_SHAPE,
-                    op + ": positions above 2^31 - 1");
+                    std::string(op) + ": positions above 2^31 - 1");
     EVKCU_CHECK_ARG(std::isfinite(d->base) && d->base > 0.0f && d->eps >= 0.0f, EVKCU_BAD_ARG,
-                    op + ": base must be positive and eps not negative");
+                    std::string(op) + ": base must be positive and eps not negative");
     EVKCU_CHECK_ARG((reinterpret_cast<uintptr_t>(d->positions) & 3u) == 0, EVKCU_BAD_ALIGN,
-                    op + ": positions must be 4-byte aligned");
+                    std::string(op) + ": positions must be 4-byte aligned");
     return EVKCU_OK;
 }
 
