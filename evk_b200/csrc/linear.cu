@@ -55,9 +55,9 @@ int operand_maps(const Product& p, CUtensorMap* ta, CUtensorMap* tb, uint32_t bo
 }
 
 // Splits of K for `tiles` slab tiles: one CTA per SM where that is possible
-// (16 x 14336 x 4096: 4 splits of 32 slabs 21.1 us, 8 23.8), else as many as
+// (16 x 14336 x 4096: 4 splits of 32 slabs 20.9 us, 8 23.8), else as many as
 // are resident; two k-blocks each at least.  A cluster of 8 packs badly where
-// a CTA takes an SM (64 x 8192 x 2048: 4 splits 14.1 us, 8 22.1).
+// a CTA takes an SM (64 x 8192 x 2048: 4 splits 13.6 us, 8 22.1).
 uint32_t slab_splits(int mr, uint64_t tiles, uint32_t kblocks, int sms) {
     const uint64_t sm = (uint64_t)sms, slots = mr == 16 ? 2 * sm : sm;
     const uint64_t most = mr == 16 ? 8 : 4, fit = tiles <= sm / 2 ? sm / tiles : slots / tiles;
@@ -166,7 +166,8 @@ int launch_pair(const Product& p, const Epi& epi) {
 
 // Which kernel a product takes: the least estimated time.  The estimates are
 // a start-and-finish cost plus rounds of tiles times k-blocks, in us (a slab CTA
-// works on one tile, so each of its rounds starts and finishes), fitted to graph-replayed runs of bf16 products with operands from HBM:
+// works on one tile, so each of its rounds starts and finishes), fitted to
+// graph-replayed runs of bf16 products with operands from HBM:
 //   M x K x N            pair 128   pair 64   slab 128 / 64   taken
 //   4096 x 2048 x 8192     90.4      104.3         -          pair 128
 //   2048 x 2048 x 2048     15.7       16.8       26.4         pair 128
@@ -318,11 +319,13 @@ constexpr uint32_t kMaxDim = 1u << 30;  // TMA coordinates are signed 32-bit
 int check_common(const char* op, uint32_t rows, uint32_t a, uint32_t b, int act, uint32_t flags, uint32_t allowed,
                  int dtype) {
     EVKCU_CHECK_ARG(dtype == EVKCU_F16 || dtype == EVKCU_BF16, EVKCU_BAD_ARG, std::string(op) + ": unknown dtype");
-    EVKCU_CHECK_ARG(act >= EVKCU_ACT_NONE && act <= EVKCU_ACT_SILU, EVKCU_BAD_ARG, std::string(op) + ": unknown activation");
+    EVKCU_CHECK_ARG(act >= EVKCU_ACT_NONE && act <= EVKCU_ACT_SILU, EVKCU_BAD_ARG,
+                    std::string(op) + ": unknown activation");
     EVKCU_CHECK_ARG((flags & ~allowed) == 0, EVKCU_BAD_ARG, std::string(op) + ": unknown flag");
     EVKCU_CHECK_ARG(a > 0 && b > 0 && a % 8 == 0 && b % 8 == 0, EVKCU_BAD_SHAPE,
                     std::string(op) + ": feature sizes must be positive multiples of 8");
-    EVKCU_CHECK_ARG(rows <= kMaxDim && a <= kMaxDim && b <= kMaxDim, EVKCU_BAD_SHAPE, std::string(op) + ": size above 2^30");
+    EVKCU_CHECK_ARG(rows <= kMaxDim && a <= kMaxDim && b <= kMaxDim, EVKCU_BAD_SHAPE,
+                    std::string(op) + ": size above 2^30");
     return EVKCU_OK;
 }
 

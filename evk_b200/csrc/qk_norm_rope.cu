@@ -445,7 +445,7 @@ int with_lph(uint32_t Dh, F&& f) {
 }
 
 // Heads x rows of a block's groups: the most heads that leave under a
-// sixteenth of the groups without one (40 heads, 16 groups: 8 x 2).
+// sixteenth of the groups without one (40 heads, 32 groups: 8 x 4).
 void set_groups(QkArgs& a, uint32_t total) {
     const uint32_t G = kThreads / lanes_per_head(a.Dh);
     for (a.GH = G; a.GH > 1; a.GH /= 2)
@@ -463,10 +463,12 @@ int check_desc(const char* op, const evkcu_qk_norm_rope_desc* d, uint32_t allowe
                     std::string(op) + ": head_dim must be a multiple of 8, 8 to 256");
     const uint32_t step = (d->flags & EVKCU_QK_HALF_SPLIT) ? 16 : 2;
     EVKCU_CHECK_ARG(d->rot_dim <= d->head_dim && (d->rot_dim ? d->rot_dim : d->head_dim) % step == 0, EVKCU_BAD_SHAPE,
-                    std::string(op) + ": rot_dim must be at most head_dim and a multiple of 2 (of 16 for half-split pairs)");
+                    std::string(op) +
+                        ": rot_dim must be at most head_dim and a multiple of 2 (of 16 for half-split pairs)");
     EVKCU_CHECK_ARG(d->heads > 0 && d->heads <= 65535 && d->kv_heads <= 65535, EVKCU_BAD_SHAPE,
                     std::string(op) + ": heads must be 1 to 65535, kv_heads at most 65535");
-    EVKCU_CHECK_ARG((uint64_t)d->batch * d->seq_len <= (1ull << 30), EVKCU_BAD_SHAPE, std::string(op) + ": more than 2^30 rows");
+    EVKCU_CHECK_ARG((uint64_t)d->batch * d->seq_len <= (1ull << 30), EVKCU_BAD_SHAPE,
+                    std::string(op) + ": more than 2^30 rows");
     EVKCU_CHECK_ARG(d->positions || (uint64_t)d->pos_offset + d->seq_len <= (1ull << 31), EVKCU_BAD_SHAPE,
                     std::string(op) + ": positions above 2^31 - 1");
     EVKCU_CHECK_ARG(std::isfinite(d->base) && d->base > 0.0f && d->eps >= 0.0f, EVKCU_BAD_ARG,
@@ -513,7 +515,8 @@ extern "C" int evkcu_qk_norm_rope(const evkcu_qk_norm_rope_desc* d, const void* 
     EVKCU_TRY(check_desc(op, d, EVKCU_QK_HALF_SPLIT | EVKCU_QK_CACHE, dtype));
     const bool cache = d->flags & EVKCU_QK_CACHE;
     EVKCU_CHECK_ARG(!cache || d->cache_len > 0, EVKCU_BAD_SHAPE, std::string(op) + ": cache_len is 0");
-    EVKCU_CHECK_ARG((v == nullptr) == (v_out == nullptr), EVKCU_BAD_ARG, std::string(op) + ": v and v_out come together");
+    EVKCU_CHECK_ARG((v == nullptr) == (v_out == nullptr), EVKCU_BAD_ARG,
+                    std::string(op) + ": v and v_out come together");
     if ((uint64_t)d->batch * d->seq_len == 0) return EVKCU_OK;
     const uint64_t qc = (uint64_t)d->heads * d->head_dim, kc = (uint64_t)d->kv_heads * d->head_dim;
     EVKCU_TRY(check_tensor(op, "q", q, d->q_pitch, qc));
@@ -599,10 +602,12 @@ extern "C" int evkcu_qk_norm_rope_backward(const evkcu_qk_norm_rope_desc* d, con
     }
     if (gains) {
         EVKCU_CHECK_ARG(workspace && workspace_bytes >= evkcu_qk_norm_rope_workspace(d->head_dim), EVKCU_BAD_ARG,
-                        std::string(op) + ": the gain gradients need a workspace of evkcu_qk_norm_rope_workspace bytes");
+                        std::string(op) +
+                            ": the gain gradients need a workspace of evkcu_qk_norm_rope_workspace bytes");
         EVKCU_CHECK_ARG(aligned16(workspace), EVKCU_BAD_ALIGN, std::string(op) + ": workspace must be 16-byte aligned");
     }
-    const uint64_t rows = (uint64_t)d->batch * d->seq_len, dh = d->head_dim, wse = gains ? 4 * kMaxPartials * dh : 0;
+    const uint64_t rows = (uint64_t)d->batch * d->seq_len, dh = d->head_dim;
+    const uint64_t wse = gains ? 4 * kMaxPartials * dh : 0;
     EVKCU_TRY(check_spans(op, {Span{"q", q, rows, d->q_pitch, qc}, Span{"k", k, rows, d->k_pitch, kc},
                                Span{"gain_q", gain_q, 1, dh, dh}, Span{"gain_k", gain_k, 1, dh, dh},
                                Span{"positions", d->positions, 1, 2 * rows, 2 * rows},
@@ -625,8 +630,10 @@ extern "C" int evkcu_qk_norm_rope_backward(const evkcu_qk_norm_rope_desc* d, con
         return with_lph(a.Dh, [&](auto lph) {
             constexpr uint32_t U = kBwdRows;
             const uint32_t R = a.GR * U, tiles = (a.rows + R - 1) / R;
-            const uint32_t grid = std::min({tiles, kMaxPartials, kBwdBlocks * (uint32_t)ds->sm_count});  // resident at once
-            const size_t smem = std::max<size_t>(4 * U * kBwdAhead * kThreads * 16 + R * angle_pitch(a.rot) * sizeof(float2),
+            // resident at once
+            const uint32_t grid = std::min({tiles, kMaxPartials, kBwdBlocks * (uint32_t)ds->sm_count});
+            const size_t smem = std::max<size_t>(4 * U * kBwdAhead * kThreads * 16 +
+                                                     R * angle_pitch(a.rot) * sizeof(float2),
                                                  gains ? (size_t)(kThreads / lph.value) * 2 * a.Dh * sizeof(float) : 0);
             auto kern = qk_backward_kernel<T, lph.value, U, kBwdAhead>;
             static std::atomic<uint64_t> done{0};

@@ -246,8 +246,10 @@ DF = [(8, 8), (64, 72), (72, 200), (264, 136), (512, 1368)]
 FFN = [(r, *DF[(i + j) % len(DF)], list(ACTS)[(i + 2 * j) % 4], DTYPES[(i + j) % 2], bool(i % 2), bool((i + j) % 3),
         bool((i // 2 + j) % 2)) for i, r in enumerate(ROWS) for j in range(3)]
 
-FFN += [(2100, 520, 1368, "silu", torch.bfloat16, True, True, False), (1001, 72, 2056, "gelu", torch.float16, True, True, True),
-        (4097, 264, 1032, "relu", torch.bfloat16, False, False, True), (300, 2056, 4104, "silu", torch.float16, True, False, False)]
+FFN += [(2100, 520, 1368, "silu", torch.bfloat16, True, True, False),
+        (1001, 72, 2056, "gelu", torch.float16, True, True, True),
+        (4097, 264, 1032, "relu", torch.bfloat16, False, False, True),
+        (300, 2056, 4104, "silu", torch.float16, True, False, False)]
 
 
 @pytest.mark.parametrize("rows,D,F,act,dt,res,pre,nk", FFN)
@@ -487,9 +489,11 @@ def qk_unit(dh):
 
 
 QK = [(1, 1, 1, 1, 8, 0, False), (2, 3, 4, 2, 16, 0, False), (3, 7, 5, 1, 32, 16, True), (1, 129, 8, 8, 64, 0, True),
-      (2, 65, 12, 4, 64, 32, True), (2, 33, 6, 3, 80, 0, True), (5, 9, 6, 2, 96, 48, False), (1, 300, 32, 8, 128, 0, False),
-      (4, 31, 7, 7, 128, 64, True), (3, 17, 4, 1, 256, 0, False), (2, 40, 3, 3, 248, 16, True), (2, 6, 2, 2, 72, 72, False),
-      (1, 2000, 2, 1, 128, 0, True), (2, 1, 200, 100, 64, 2, False)]
+      (2, 65, 12, 4, 64, 32, True), (2, 33, 6, 3, 80, 0, True), (5, 9, 6, 2, 96, 48, False),
+      (1, 300, 32, 8, 128, 0, False), (4, 31, 7, 7, 128, 64, True), (3, 17, 4, 1, 256, 0, False),
+      (2, 40, 3, 3, 248, 16, True), (2, 6, 2, 2, 72, 72, False), (1, 2000, 2, 1, 128, 0, True),
+      (2, 1, 200, 100, 64, 2, False), (2, 50, 3, 2, 128, 96, True), (1, 5000, 20, 4, 64, 48, True),
+      (3, 2500, 12, 12, 128, 0, False)]
 
 
 @pytest.mark.parametrize("B,S,H,Hk,dh,rot,half", QK)

@@ -111,7 +111,8 @@ DESC_REFUSALS = [
 
 @pytest.mark.parametrize("kw,status", DESC_REFUSALS + [
     (dict(flags=2), SHAPE), (dict(flags=4), ARG), (dict(v=P[6]), ARG), (dict(vo=P[7]), ARG),
-    (dict(qo=None), ARG), (dict(ko=None), ARG), (dict(v=P[6], vo=P[7] + 8), ALIGN), (dict(v=P[6], vo=P[7], v_pitch=64), SHAPE),
+    (dict(qo=None), ARG), (dict(ko=None), ARG), (dict(v=P[6], vo=P[7] + 8), ALIGN),
+    (dict(v=P[6], vo=P[7], v_pitch=64), SHAPE),
     (dict(qo=P[0]), ARG), (dict(ko=P[1]), ARG), (dict(qo=P[5]), ARG), (dict(ko=P[2], gk=None), ARG),
     (dict(flags=2, cache_len=5, ko=P[1], k_pitch=128), ARG), (dict(batch=0), OK), (dict(seq_len=0), OK),
 ])
