@@ -531,7 +531,8 @@ def test_qk_norm_rope(B, S, H, Hk, dh, rot, half, dt, form):
 
 
 @pytest.mark.parametrize("dt", DTYPES)
-@pytest.mark.parametrize("B,S,H,Hk,dh,cache_len", [(8, 1, 32, 8, 128, 100), (3, 5, 4, 4, 64, 37), (1, 1, 1, 1, 80, 3)])
+@pytest.mark.parametrize("B,S,H,Hk,dh,cache_len", [(8, 1, 32, 8, 128, 100), (3, 5, 4, 4, 64, 37), (1, 1, 1, 1, 80, 3),
+                                                    (3, 2000, 8, 8, 128, 2100)])
 def test_qk_norm_rope_into_a_cache(B, S, H, Hk, dh, cache_len, dt):
     g = gen(cache_len)
     qkv = rnd(g, dt, B, S, (H + 2 * Hk) * dh)
