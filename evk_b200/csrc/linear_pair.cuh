@@ -413,7 +413,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 }
             }
         }
-        if (lane == 0) tma_store_wait_read<0>();  // the boxes outlive the stores' reads
+        if (lane == 0) tma_store_wait_all();  // written, not only read, before the CTA counts as done
         tc_fence_before();
     }
     __syncthreads();
