@@ -14,9 +14,10 @@
 // 0) into one of two accumulators, so that an epilogue overlaps the next
 // tile's MMAs, and warps 2-9 epilogue.  Each epilogue warp works alone on 32
 // rows x 32 columns at a time (its TMEM lane quarter, alternate chunks with
-// the other warp of that quarter) through two or four 2 KB boxes of its own: inputs
-// (residual, saved pre-activations) arrive and outputs leave by TMA in the
-// 64-byte swizzle, inputs one chunk ahead where the boxes allow, and only warp barriers order them.
+// the other warp of that quarter) through two or four 2 KB boxes of its own:
+// inputs (residual, saved pre-activations) arrive and outputs leave by TMA in
+// the 64-byte swizzle, inputs one chunk ahead where the boxes allow, and only
+// warp barriers order them.
 // Groups of four warps sharing boxes behind named barriers were no faster, and
 // a warp that gave up waiting would have left the others in the barrier.
 // No load is multicast.  All waits are bounded.
