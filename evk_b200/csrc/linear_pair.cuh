@@ -357,6 +357,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             int got = 0;
             if (lane == 0) got = (int)mbar_wait(&tfull[buf], (j >> 1) & 1, s_abort, err, kTimeout);
             live = __shfl_sync(0xffffffffu, got, 0) != 0;
+            __syncwarp();  // a shuffle orders no memory: what lane 0 waited for, the others may read after this
             if (!live) {
                 if (nin && lane == 0) mbar_drain(wbar + n % sets, (n / sets) & 1);
                 break;
@@ -385,6 +386,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     got = 0;
                     if (lane == 0) got = (int)mbar_wait(wbar + n % sets, (n / sets) & 1, s_abort, err, kTimeout);
                     live = __shfl_sync(0xffffffffu, got, 0) != 0;
+                    __syncwarp();  // lane 0 has seen the inputs arrive and the set's other box free
                     if (!live) {
                         if (lane == 0) {
                             mbar_drain(wbar + n % sets, (n / sets) & 1);

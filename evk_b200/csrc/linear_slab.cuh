@@ -179,6 +179,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<MR>::PER_SM)
         const int q = warp & 3;  // TMEM lane quarter: output columns 32 q + lane
         const bool ok = __shfl_sync(0xffffffffu,
                                     lane == 0 ? (int)mbar_wait_sleep(accum, 0, s_abort, err, kTimeout) : 0, 0) != 0;
+        __syncwarp();  // a shuffle orders no memory: what lane 0 waited for, the others may read after this
         tc_fence_after();
         if (ok) {
             float* col = stage + q * 32 + lane;

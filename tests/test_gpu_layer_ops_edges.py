@@ -1,0 +1,39 @@
+"""Edges of evkcu_linear, evkcu_gated_ffn and evkcu_qk_norm_rope that
+test_gpu_layer_ops.py does not reach, with its helpers and bounds."""
+import pytest
+import torch
+
+import evk_b200 as evk
+from test_gpu_layer_ops import DTYPES, check, ffn_back_ref, gen, lin_ref, rnd, rounded
+
+pytestmark = pytest.mark.gpu
+
+
+# -------------------------------------------- order of loads, stores, waits --
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("rows,D,F", [(1030, 520, 2056), (2305, 264, 1032)])
+def test_staged_inputs_arrive_before_they_are_read(rows, D, F, dt):
+    """Epilogues that load boxes (residual, saved pre-activations, gradients
+    added to) in the large-product kernel, several tiles a CTA: right, and the
+    same bits in every call."""
+    g = gen(rows + D)
+    x, wi, wo = rnd(g, dt, rows, D), rnd(g, dt, D, 2 * F, std=F ** -0.5), rnd(g, dt, F, D, std=D ** -0.5)
+    z, dy, res = rnd(g, dt, rows, 2 * F), rnd(g, dt, rows, D), rnd(g, dt, rows, 2 * F)
+    old = rnd(g, dt, rows, D)
+    first = None
+    for _ in range(6):
+        dz, y, pre, dx = torch.empty_like(z), res.clone(), torch.empty_like(z), old.clone()
+        evk.linear(x, wi, y, residual=y, act=evk.ACT_GELU, pre=pre)
+        evk.gated_ffn_backward(x, wi, wo, z, dy, dz, None, dx=dx, acc=True)
+        got = [y, pre, dz, dx]
+        if first is None:
+            first = got
+        assert all(torch.equal(a, b) for a, b in zip(got, first))
+    evk.check_device_error()
+    zr, ez, yr, tol = lin_ref(x, wi, None, res, "gelu", dt)
+    check(first[0], yr, tol, "y")
+    check(first[1], zr, rounded(zr, ez, dt), "pre")
+    (dzr, ez), _, (dxr, edx), _, _ = ffn_back_ref(x, wi, wo, z, dy, "silu", dt)
+    check(first[2], dzr, ez, "dpre")
+    dxr = dxr + old.double()
+    check(first[3], dxr, rounded(dxr, edx + 2.0 ** -23 * dxr.abs(), dt), "dx")
