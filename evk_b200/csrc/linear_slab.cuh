@@ -216,7 +216,8 @@ __global__ void __launch_bounds__(THREADS, Cfg<MR>::PER_SM)
         const uint32_t base = smem_u32(stage), n = r1 > r0 ? (r1 - r0) * Q : 0;
         for (uint32_t i0 = threadIdx.x; i0 < n; i0 += 2 * THREADS) {
             float sum[2][4] = {};
-            const uint32_t i1 = min(i0 + THREADS, n - 1);
+            // without a second piece the first again: any other is being written by its own thread
+            const uint32_t i1 = i0 + THREADS < n ? i0 + THREADS : i0;
             const uint32_t at[2] = {base + ((r0 + i0 / Q) * LD + i0 % Q * 4) * 4,
                                     base + ((r0 + i1 / Q) * LD + i1 % Q * 4) * 4};
             for (uint32_t p0 = 0; p0 < splits; p0 += 4) {  // in rank order

@@ -37,3 +37,22 @@ def test_staged_inputs_arrive_before_they_are_read(rows, D, F, dt):
     check(first[2], dzr, ez, "dpre")
     dxr = dxr + old.double()
     check(first[3], dxr, rounded(dxr, edx + 2.0 ** -23 * dxr.abs(), dt), "dx")
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("rows,K,N", [(3, 2048, 264), (13, 1024, 136), (16, 4096, 520), (21, 2048, 264),
+                                      (63, 1024, 136), (64, 4096, 264), (101, 2048, 136), (127, 4096, 264)])
+def test_split_sums(rows, K, N, dt):
+    """Products of few tiles, K split over a cluster whose CTAs share out rows
+    that do not divide evenly: right, and the same bits in every call."""
+    g = gen(rows + K)
+    x, w = rnd(g, dt, rows, K), rnd(g, dt, K, N, std=K ** -0.5)
+    first = None
+    for _ in range(6):
+        y = torch.empty(rows, N, dtype=dt, device="cuda")
+        evk.linear(x, w, y)
+        first = y if first is None else first
+        assert torch.equal(y, first)
+    evk.check_device_error()
+    _, _, yr, tol = lin_ref(x, w, None, None, "none", dt)
+    check(first, yr, tol, "y")
