@@ -242,7 +242,8 @@ __global__ void __cluster_dims__(1, kDactCluster, 1) __launch_bounds__(kDactThre
             Vec8 a[U], z[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const uint64_t at = (uint64_t)min(r + u * RL, r1 - 1) * N + col;
+                // past the end its first row again: others may be writing theirs (dz may be dy or pre)
+                const uint64_t at = (uint64_t)(r + u * RL < r1 ? r + u * RL : r) * N + col;
                 a[u] = ld_vec8(dy + at);
                 if (act != EVKCU_ACT_NONE) z[u] = ld_vec8(pre + at);
             }

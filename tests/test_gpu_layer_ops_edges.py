@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import evk_b200 as evk
-from test_gpu_layer_ops import DTYPES, check, ffn_back_ref, gen, lin_ref, rnd, rounded
+from test_gpu_layer_ops import DTYPES, back_ref, check, ffn_back_ref, gen, lin_ref, rnd, rounded
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +56,24 @@ def test_split_sums(rows, K, N, dt):
     evk.check_device_error()
     _, _, yr, tol = lin_ref(x, w, None, None, "none", dt)
     check(first, yr, tol, "y")
+
+
+@pytest.mark.parametrize("rows", [1, 3, 9, 515, 1031])
+@pytest.mark.parametrize("where", ["pre", "dy"])
+def test_activation_gradient_in_place_of_ragged_rows(rows, where):
+    """dpre over pre or over dy, rows that leave lanes without a row: the bits
+    of separate buffers, and the column sums of the unrounded values."""
+    dt, g, K, N = torch.bfloat16, gen(rows), 72, 136
+    x, w = rnd(g, dt, rows, K), rnd(g, dt, K, N, std=N ** -0.5)
+    z, dy = rnd(g, dt, rows, N), rnd(g, dt, rows, N)
+    dz, dx, db = torch.empty_like(z), torch.empty_like(x), torch.empty(N, dtype=dt, device="cuda")
+    evk.linear_backward(x, w, dy, dx=dx, dbias=db, act=evk.ACT_SILU, pre=z, dpre=dz)
+    dzr, ez, (dxr, edx), _, (dbr, edb) = back_ref(x, w, z, dy, "silu", dt)
+    check(dz, dzr, ez, "dpre")
+    check(dx, dxr, rounded(dxr, edx, dt), "dx")
+    check(db, dbr, rounded(dbr, edb, dt), "dbias")
+    for _ in range(4):
+        zz, dd, d2, b2 = z.clone(), dy.clone(), torch.empty_like(x), torch.empty_like(db)
+        over = zz if where == "pre" else dd
+        evk.linear_backward(x, w, dd, dx=d2, dbias=b2, act=evk.ACT_SILU, pre=zz, dpre=over)
+        assert torch.equal(over, dz) and torch.equal(d2, dx) and torch.equal(b2, db)
