@@ -290,6 +290,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 if (++s == STAGES) s = 0, ph ^= 1;
             }
         }
+        // The last releases of the slots have arrived before the CTA leaves.
+        for (uint32_t i = issued > STAGES ? issued - STAGES : 0; ok && i < issued; ++i)
+            ok = mbar_wait(&empty[i % STAGES], (i / STAGES) & 1, s_abort, err, kTimeout);
     } else if (warp == 1) {
         if (rank == 0) {
             const bool leader = elect_one();
@@ -380,7 +383,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 if (i + 1 == CHUNKS) {  // the warp's part of the accumulator is in registers
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive_relaxed(map_shared_rank(&tempty[buf], 0));
+                    // Only arrivals that a later tile waits for: rank 0 may leave before any other lands.
+                    if (lane == 0 && t + 2 * npairs < total) mbar_arrive_relaxed(map_shared_rank(&tempty[buf], 0));
                 }
                 if (nin) {
                     got = 0;

@@ -149,6 +149,10 @@ __global__ void __launch_bounds__(THREADS, Cfg<MR>::PER_SM)
             }
             if (++s == STAGES) s = 0, ph ^= 1;
         }
+        // The last releases of the slots have arrived before the CTA leaves.
+        bool ok = issued == nkb;
+        for (uint32_t i = issued > STAGES ? issued - STAGES : 0; ok && i < issued; ++i)
+            ok = mbar_wait(&empty[i % STAGES], (i / STAGES) & 1, s_abort, err, kTimeout);
     } else if (warp == 1) {
         const bool leader = elect_one();
         bool ok = true;

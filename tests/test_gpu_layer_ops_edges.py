@@ -77,3 +77,27 @@ def test_activation_gradient_in_place_of_ragged_rows(rows, where):
         over = zz if where == "pre" else dd
         evk.linear_backward(x, w, dd, dx=d2, dbias=b2, act=evk.ACT_SILU, pre=zz, dpre=over)
         assert torch.equal(over, dz) and torch.equal(d2, dx) and torch.equal(b2, db)
+
+
+def test_many_small_products_back_to_back():
+    """Short products one behind the other, so that a kernel starts where the
+    one before has just left: equal bits to each call alone."""
+    dt, g = torch.bfloat16, gen(17)
+    calls = []
+    for rows, K, N in ((300, 8, 2056), (1030, 64, 520), (5, 72, 264), (2305, 136, 1032), (40, 264, 136)):
+        x, w = rnd(g, dt, rows, K), rnd(g, dt, K, N, std=K ** -0.5)
+        r = rnd(g, dt, rows, N)
+        y = torch.empty_like(r)
+        evk.linear(x, w, y, residual=r)
+        torch.cuda.synchronize()
+        _, _, yr, tol = lin_ref(x, w, None, r, "none", dt)
+        check(y, yr, tol, "y")
+        calls.append((x, w, r, y))
+    outs = []
+    for _ in range(40):
+        for x, w, r, _ in calls:
+            outs.append(torch.empty_like(r))
+            evk.linear(x, w, outs[-1], residual=r)
+    evk.check_device_error()
+    for i, o in enumerate(outs):
+        assert torch.equal(o, calls[i % len(calls)][3])
