@@ -350,7 +350,9 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) qk_backward_kernel(const
 #pragma unroll
                     for (int e = 0; e < 8; ++e) ss += x[v][e] * x[v][e];
                 }
-                const float r = rsqrtf(group_sum<LPH>(ss) * a.inv_dh + a.eps);
+                // A group without a head or row works on zeros: with eps = 0 its r would be infinite.
+                const bool live = on && rl < nrows;
+                const float ms = group_sum<LPH>(ss) * a.inv_dh + a.eps, r = live ? rsqrtf(ms) : 0.0f;
                 rotate<LPH>(a, s_cs + min(rl, nrows - 1) * pitch, c, -1.0f, t);
 #pragma unroll
                 for (int v = 0; v < 2; ++v)
@@ -367,8 +369,8 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) qk_backward_kernel(const
 #pragma unroll
                     for (int e = 0; e < 8; ++e) t[v][e] = r * (t[v][e] - x[v][e] * m);
                 T* p = dst + (row0 + rl) * opitch;
-                if (on && rl < nrows && lane0) st_vec8(p, pack8<T>(t[0]));
-                if (on && rl < nrows && lane1) st_vec8(p + LPH * 8, pack8<T>(t[1]));
+                if (live && lane0) st_vec8(p, pack8<T>(t[0]));
+                if (live && lane1) st_vec8(p + LPH * 8, pack8<T>(t[1]));
             }
             if (++cur == LA) cur = 0;
             request();

@@ -4,7 +4,8 @@ import pytest
 import torch
 
 import evk_b200 as evk
-from test_gpu_layer_ops import DTYPES, back_ref, check, ffn_back_ref, gen, lin_ref, rnd, rounded
+from test_gpu_layer_ops import (DTYPES, back_ref, check, ffn_back_ref, gen, lin_ref, qk_ref, qk_unit, rnd,
+                                rounded)
 
 pytestmark = pytest.mark.gpu
 
@@ -101,3 +102,46 @@ def test_many_small_products_back_to_back():
     evk.check_device_error()
     for i, o in enumerate(outs):
         assert torch.equal(o, calls[i % len(calls)][3])
+
+
+# ------------------------------------------------------------- qk_norm_rope --
+def qk_grad_ref(x, dy, heads, gain, pos, rot, half, eps):
+    """(dx, its bound before rounding, dgain, its bound before rounding): the
+    formulas and bounds of test_qk_norm_rope_backward."""
+    _, n, r, w, rotate, spread = qk_ref(x, heads, gain, pos, rot, half, 10000.0, eps)
+    dy = dy.double().reshape(n.shape)
+    t = rotate(dy, -1.0)
+    dn = t * w
+    su, e = spread(dy), 2 * qk_unit(n.shape[-1])
+    mabs = (su * w.abs() * n.abs()).mean(-1, keepdim=True)
+    dx = r * (dn - n * (dn * n).mean(-1, keepdim=True))
+    count = n.shape[0] * n.shape[1] * n.shape[2]
+    return (dx, 4 * e * r * (su * w.abs() + n.abs() * mabs), (t * n).sum((0, 1, 2)),
+            (2 * e + min(count, 2048) * 2.0 ** -23) * (su * n.abs()).sum((0, 1, 2)))
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("eps", [0.0, 1e-30])
+@pytest.mark.parametrize("B,S,H,Hk,dh,rot,half", [(1, 1, 32, 8, 128, 0, False), (1, 1001, 32, 8, 128, 0, False),
+                                                  (3, 7, 5, 1, 32, 16, True), (2, 33, 6, 3, 80, 0, True),
+                                                  (1, 2, 3, 0, 256, 0, False)])
+def test_gain_gradients_without_eps(B, S, H, Hk, dh, rot, half, eps, dt):
+    """eps = 0, no head all zeros, rows and heads that leave groups of a block
+    idle: gain gradients of the real rows alone."""
+    g = gen(B * 10 + S + dh)
+    dt_k = Hk * dh
+    q, k = rnd(g, dt, B, S, H * dh, std=2.0), rnd(g, dt, B, S, dt_k, std=2.0) if Hk else None
+    dqo, dko = rnd(g, dt, B, S, H * dh), rnd(g, dt, B, S, dt_k) if Hk else None
+    gq, gk = (rnd(g, dt, dh, std=0.2, mean=1.0) for _ in range(2))
+    dgq, dgk = torch.empty_like(gq), torch.empty_like(gk)
+    dq, dk = torch.empty_like(q), torch.empty_like(k) if Hk else None
+    ws = torch.empty(evk.qk_norm_rope_workspace(dh), dtype=torch.uint8, device="cuda")
+    evk.qk_norm_rope_backward(q, k, dqo, dko, dq, dk, H, gain_q=gq, gain_k=gk if Hk else None, dgain_q=dgq,
+                              dgain_k=dgk if Hk else None, workspace=ws, rot_dim=rot, half_split=half, eps=eps)
+    pos = torch.arange(S, device="cuda")[None].expand(B, S)
+    for x, dy, heads, gain, dx, dg in ((q, dqo, H, gq, dq, dgq), (k, dko, Hk, gk, dk, dgk)):
+        if x is None:
+            continue
+        xr, ex, gr, eg = qk_grad_ref(x, dy, heads, gain, pos, rot, half, eps)
+        check(dx.reshape(xr.shape), xr, rounded(xr, ex, dt), "dx")
+        check(dg, gr, rounded(gr, eg, dt), "dgain")
