@@ -69,8 +69,8 @@ __device__ __forceinline__ float2 turn_cs(double turns, int32_t pos) {
     return make_float2(__cosf(x), __sinf(x));
 }
 
-// Row pitch of the angles: whole lanes of four pairs, the pairs past rot / 2
-// turned by 0 so that a lane need not look where the rotation ends.
+// Row pitch of the angles: whole lanes of four pairs, so that each lane's are
+// aligned.  What lies past rot / 2 is not used.
 __host__ __device__ inline uint32_t angle_pitch(uint32_t rot) { return (rot / 2 + 3) / 4 * 4; }
 
 // The table lies among the kernel's parameters.  Lanes read different entries,
@@ -86,17 +86,21 @@ __device__ __forceinline__ void fill_angles(const QkArgs& a, float2* cs, uint32_
     const uint32_t pitch = angle_pitch(a.rot);
     for (uint32_t i = threadIdx.x; i < nrows * pitch; i += kThreads) {
         const uint32_t p = i % pitch;
-        cs[i] = p < a.rot / 2 ? turn_cs(turns_at(a, p), position(a, row0 + i / pitch)) : make_float2(1.0f, 0.0f);
+        if (p < a.rot / 2) cs[i] = turn_cs(turns_at(a, p), position(a, row0 + i / pitch));
     }
 }
 
-// One vector of eight elements rotated by four (cos, sin) pairs.
-__device__ __forceinline__ void rotate_pairs(const float2* cs, float sgn, float (&f)[8]) {
+// One vector of eight elements rotated by four (cos, sin) pairs; TAIL: only its
+// first `pairs` pairs.  (Turning the others by 0 would pass an infinity or NaN
+// on to its neighbour, as 0 times it.)
+template <bool TAIL>
+__device__ __forceinline__ void rotate_pairs(const float2* cs, float sgn, float (&f)[8], uint32_t pairs) {
     const float4* v = reinterpret_cast<const float4*>(cs);
     const float4 t0 = v[0], t1 = v[1];
     const float co[4] = {t0.x, t0.z, t1.x, t1.z}, si[4] = {t0.y, t0.w, t1.y, t1.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
+        if (TAIL && j >= pairs) break;
         const float x = f[2 * j], y = f[2 * j + 1], s = sgn * si[j];
         f[2 * j] = x * co[j] - y * s;
         f[2 * j + 1] = x * s + y * co[j];
@@ -116,13 +120,16 @@ __device__ __forceinline__ void rotate_halves(const float2* cs, float s0, const 
 // Rotates the lane's two vectors, c and c + LPH of the head's, by the row's
 // angles cs (see angle_pitch); sgn = -1 is the inverse rotation.  All lanes of
 // the warp call it together: half-split pairs are vectors n and n + hl, the
-// lane's own two where hl = LPH, otherwise exchanged.
-template <int LPH>
+// lane's own two where hl = LPH, otherwise exchanged.  TAIL: the rotated part ends
+// inside a vector (adjacent pairs only).  A template and not a branch: with the
+// test in every kernel 16384 rows of 32 heads of 128 took 55 us instead of 53.
+template <int LPH, bool TAIL>
 __device__ __forceinline__ void rotate(const QkArgs& a, const float2* cs, uint32_t c, float sgn, float (&f)[2][8]) {
     if (!a.half_split) {
 #pragma unroll
         for (int v = 0; v < 2; ++v)
-            if ((c + v * LPH) * 8 < a.rot) rotate_pairs(cs + (c + v * LPH) * 4, sgn, f[v]);
+            if ((c + v * LPH) * 8 < a.rot)
+                rotate_pairs<TAIL>(cs + (c + v * LPH) * 4, sgn, f[v], a.rot / 2 - (c + v * LPH) * 4);
         return;
     }
     const uint32_t hl = a.rot / 16;
@@ -194,7 +201,7 @@ __device__ __forceinline__ void cp_wait() {
 // A block walks row tiles b, b + gridDim.x, ... in rounds of one head of U
 // rows a group; the copies of the next LA rounds, running on from one tile
 // into the next, are in flight while one is worked on.
-template <typename T, int LPH, int U, int LA>
+template <typename T, int LPH, int U, int LA, bool TAIL>
 __global__ void __launch_bounds__(kThreads, U == 1 ? 4 : kFwdBlocks)
     qk_forward_kernel(const __grid_constant__ QkArgs a) {
     extern __shared__ __align__(16) uint8_t s_raw[];
@@ -261,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, U == 1 ? 4 : kFwdBlocks)
                     f[0][e] *= r * w[0][e];
                     f[1][e] *= r * w[1][e];
                 }
-                rotate<LPH>(a, s_cs + min(rl, nrows - 1) * pitch, c, 1.0f, f);
+                rotate<LPH, TAIL>(a, s_cs + min(rl, nrows - 1) * pitch, c, 1.0f, f);
                 bool st = on && rl < nrows;
                 uint64_t at = row;
                 if (a.cache && !is_q && st) {
@@ -283,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, U == 1 ? 4 : kFwdBlocks)
 // meets, the block adds its groups in order and stores one partial row, and
 // qk_gain_kernel adds the partials in order, so the sums do not depend on
 // timing.
-template <typename T, int LPH, int U, int LA>
+template <typename T, int LPH, int U, int LA, bool TAIL>
 __global__ void __launch_bounds__(kThreads, kBwdBlocks) qk_backward_kernel(const __grid_constant__ QkArgs a) {
     extern __shared__ __align__(16) uint8_t s_raw[];
     Vec8* slot = reinterpret_cast<Vec8*>(s_raw) + threadIdx.x;  // [LA U][x, dy][2][kThreads]
@@ -353,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) qk_backward_kernel(const
                 // A group without a head or row works on zeros: with eps = 0 its r would be infinite.
                 const bool live = on && rl < nrows;
                 const float ms = group_sum<LPH>(ss) * a.inv_dh + a.eps, r = live ? rsqrtf(ms) : 0.0f;
-                rotate<LPH>(a, s_cs + min(rl, nrows - 1) * pitch, c, -1.0f, t);
+                rotate<LPH, TAIL>(a, s_cs + min(rl, nrows - 1) * pitch, c, -1.0f, t);
 #pragma unroll
                 for (int v = 0; v < 2; ++v)
 #pragma unroll
@@ -444,6 +451,15 @@ int with_lph(uint32_t Dh, F&& f) {
         case 8: return f(std::integral_constant<int, 8>());
         default: return f(std::integral_constant<int, 16>());
     }
+}
+
+// The same with whether the rotated part ends inside a vector of eight.
+template <class F>
+int with_layout(const QkArgs& a, F&& f) {
+    return with_lph(a.Dh, [&](auto lph) {
+        if (a.rot % 8 != 0) return f(lph, std::true_type());
+        return f(lph, std::false_type());
+    });
 }
 
 // Heads x rows of a block's groups: the most heads that leave under a
@@ -558,12 +574,12 @@ extern "C" int evkcu_qk_norm_rope(const evkcu_qk_norm_rope_desc* d, const void* 
     const bool large = ((uint64_t)a.rows + a.GR * kFwdRows - 1) / (a.GR * kFwdRows) >= 2 * (uint64_t)ds->sm_count;
     a.heads_per_block = large ? total : a.GH;
     return EVKCU_DISPATCH_DTYPE(dtype, T, [&] {
-        return with_lph(a.Dh, [&](auto lph) {
+        return with_layout(a, [&](auto lph, auto tail) {
             const uint32_t R = a.GR * (large ? kFwdRows : 1), tiles = (a.rows + R - 1) / R;
             const size_t smem = 2 * (large ? kFwdRows * kFwdAhead : 1) * kThreads * 16 +
                                 R * angle_pitch(a.rot) * sizeof(float2);
-            auto kern = large ? qk_forward_kernel<T, lph.value, kFwdRows, kFwdAhead>
-                              : qk_forward_kernel<T, lph.value, 1, 1>;
+            auto kern = large ? qk_forward_kernel<T, lph.value, kFwdRows, kFwdAhead, tail.value>
+                              : qk_forward_kernel<T, lph.value, 1, 1, tail.value>;
             static std::atomic<uint64_t> done[2];
             EVKCU_TRY(allow_smem(kern, kMaxSmem, done[large]));
             const dim3 grid(large ? std::min(tiles, kFwdBlocks * (uint32_t)ds->sm_count) : tiles,
@@ -629,7 +645,7 @@ extern "C" int evkcu_qk_norm_rope_backward(const evkcu_qk_norm_rope_desc* d, con
     a.partial = gains ? (float*)workspace : nullptr;
     set_groups(a, a.H + a.Hk);
     return EVKCU_DISPATCH_DTYPE(dtype, T, [&] {
-        return with_lph(a.Dh, [&](auto lph) {
+        return with_layout(a, [&](auto lph, auto tail) {
             constexpr uint32_t U = kBwdRows;
             const uint32_t R = a.GR * U, tiles = (a.rows + R - 1) / R;
             // resident at once
@@ -637,7 +653,7 @@ extern "C" int evkcu_qk_norm_rope_backward(const evkcu_qk_norm_rope_desc* d, con
             const size_t smem = std::max<size_t>(4 * U * kBwdAhead * kThreads * 16 +
                                                      R * angle_pitch(a.rot) * sizeof(float2),
                                                  gains ? (size_t)(kThreads / lph.value) * 2 * a.Dh * sizeof(float) : 0);
-            auto kern = qk_backward_kernel<T, lph.value, U, kBwdAhead>;
+            auto kern = qk_backward_kernel<T, lph.value, U, kBwdAhead, tail.value>;
             static std::atomic<uint64_t> done{0};
             EVKCU_TRY(allow_smem(kern, kMaxSmem, done));
             kern<<<grid, kThreads, smem, st>>>(a);

@@ -145,3 +145,30 @@ def test_gain_gradients_without_eps(B, S, H, Hk, dh, rot, half, eps, dt):
         xr, ex, gr, eg = qk_grad_ref(x, dy, heads, gain, pos, rot, half, eps)
         check(dx.reshape(xr.shape), xr, rounded(xr, ex, dt), "dx")
         check(dg, gr, rounded(gr, eg, dt), "dgain")
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("rot", [2, 20, 30, 70])
+@pytest.mark.parametrize("bad", ["inf", "nan"])
+def test_unrotated_values_stay_apart(rot, bad, dt):
+    """A rotated part that ends inside a vector of eight: values past it keep
+    to themselves, so an infinity or NaN in one column of a gradient reaches
+    no other column's gain gradient, nor in a gain another column's output."""
+    g, dh, S, H = gen(rot), 80, 5, 3
+    x, dy = rnd(g, dt, 1, S, H * dh), rnd(g, dt, 1, S, H * dh)
+    gain, dgain, dx = rnd(g, dt, dh, std=0.2, mean=1.0), torch.empty(dh, dtype=dt, device="cuda"), torch.empty_like(x)
+    ws = torch.empty(evk.qk_norm_rope_workspace(dh), dtype=torch.uint8, device="cuda")
+    pos = torch.arange(S, device="cuda")[None]
+    _, _, gr, eg = qk_grad_ref(x, dy, H, gain, pos, rot, False, 1e-5)
+    yr, n, _, w, _, spread = qk_ref(x, H, gain, pos, rot, False, 10000.0, 1e-5)
+    tol = rounded(yr, 2 * qk_unit(dh) * spread(n * w), dt)
+    dyb, gainb, y = dy.clone(), gain.clone(), torch.empty_like(x)
+    dyb.view(1, S, H, dh)[0, 2, 1, rot] = float(bad)
+    gainb[rot] = float(bad)
+    evk.qk_norm_rope_backward(x, None, dyb, None, dx, None, H, gain_q=gain, dgain_q=dgain, workspace=ws, rot_dim=rot)
+    evk.qk_norm_rope(x, None, y, None, H, gain_q=gainb, rot_dim=rot)
+    keep = [i for i in range(dh) if i != rot]
+    check(dgain[keep], gr[keep], rounded(gr, eg, dt)[keep], "dgain")
+    assert not bool(torch.isfinite(dgain[rot]))
+    check(y.reshape(yr.shape)[..., keep], yr[..., keep], tol[..., keep], "y")
+    assert not bool(torch.isfinite(y.reshape(yr.shape)[..., rot]).any())
