@@ -242,8 +242,10 @@ __global__ void __cluster_dims__(1, kDactCluster, 1) __launch_bounds__(kDactThre
             Vec8 a[U], z[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                // past the end its first row again: others may be writing theirs (dz may be dy or pre)
-                const uint64_t at = (uint64_t)(r + u * RL < r1 ? r + u * RL : r) * N + col;
+                // past the end its first row again: others may be writing theirs (dz may be dy or pre).
+                // At U = 1 min is r, but the compiler spills less with it (4096 x 8192: 41.5 us, not 43.5).
+                const uint32_t row = U == 1 ? min(r, r1 - 1) : r + u * RL < r1 ? r + u * RL : r;
+                const uint64_t at = (uint64_t)row * N + col;
                 a[u] = ld_vec8(dy + at);
                 if (act != EVKCU_ACT_NONE) z[u] = ld_vec8(pre + at);
             }
