@@ -74,9 +74,19 @@ inline int check_ptr(const char* op, const char* name, const void* p, bool requi
     return EVKCU_OK;
 }
 
-// sigmoid from ex2 and a reciprocal: relative error below 2^-20, so the
-// activations below are exact to well under a 2-byte rounding.
-__device__ __forceinline__ float sigmoid_f(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+// 1 / (1 + 2^(-z log2 e)) from ex2 and a reciprocal, both sides of the quotient
+// scaled by 2^-16: unscaled, the exponential and its reciprocal leave fp32 below
+// z = -87, where z sigmoid(z) = -1e-36 is still a normal bf16 value; scaled, only
+// past z = -98, where it is below half of bf16's smallest step.  Relative error at
+// most (9 + 0.6 |z|) 2^-23: the scaled exponent's rounding (half a step at 16, and
+// what log2 e and the product leave), 2 units of ex2 and 1 of the reciprocal.  So
+// the activations below are exact to well under a 2-byte rounding.
+__device__ __forceinline__ float sigmoid_f(float z) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(z, -1.4426950408889634f, -16.0f)));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e + 0x1p-16f));
+    return 0x1p-16f * r;
+}
 
 constexpr float kGeluA = 1.5957691216057308f;  // 2 sqrt(2 / pi)
 constexpr float kGeluB = 0.044715f;

@@ -1,10 +1,12 @@
 """Edges of evkcu_linear, evkcu_gated_ffn and evkcu_qk_norm_rope that
 test_gpu_layer_ops.py does not reach, with its helpers and bounds."""
+import math
+
 import pytest
 import torch
 
 import evk_b200 as evk
-from test_gpu_layer_ops import (DTYPES, back_ref, check, ffn_back_ref, gen, lin_ref, qk_ref, qk_unit, rnd,
+from test_gpu_layer_ops import (ACTS, DTYPES, back_ref, check, ffn_back_ref, gen, lin_ref, qk_ref, qk_unit, rnd,
                                 rounded)
 
 pytestmark = pytest.mark.gpu
@@ -172,3 +174,36 @@ def test_unrotated_values_stay_apart(rot, bad, dt):
     assert not bool(torch.isfinite(dgain[rot]))
     check(y.reshape(yr.shape)[..., keep], yr[..., keep], tol[..., keep], "y")
     assert not bool(torch.isfinite(y.reshape(yr.shape)[..., rot]).any())
+
+
+# --------------------------------------------------------------- activations --
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("dt", DTYPES)
+def test_activations_of_far_negative_values(act, dt):
+    """Where exp(v) leaves fp32's normal range, v the sigmoid's argument, the
+    result is still one of the storage type for a while: every value and
+    derivative from -4 down.
+
+    Relative error of the sigmoid there: the exponential's 2 + 1.2 |v| units of
+    2^-23, 6 for the quotient and the products behind it, and for GELU six
+    roundings of v itself, 3 |v| units; the derivatives' two terms of opposite
+    sign stand 1 to 3.9 at least, (3.9 + 1) / (3.9 - 1) < 2."""
+    lo = -100.0 if act == "silu" else -14.0
+    z = torch.linspace(-4.0, lo, 8 * 4096, device="cuda").to(dt).view(512, 64)
+    arg = z.double() if act == "silu" else math.sqrt(8 / math.pi) * (z.double() + 0.044715 * z.double() ** 3)
+    rel = (8 + (1.2 if act == "silu" else 4.2) * arg.abs()) * 2.0 ** -23
+    eye = torch.eye(64, dtype=dt, device="cuda")
+    y = torch.empty_like(z)
+    evk.linear(z, eye, y, act=ACTS[act])  # z itself is the product
+    ref = act64_far(z.double(), act)
+    check(y, ref, rounded(ref, rel * ref.abs(), dt), "act")
+    dz, db = torch.empty_like(z), torch.empty(64, dtype=dt, device="cuda")
+    evk.linear_backward(z, eye, torch.ones_like(z), dbias=db, act=ACTS[act], pre=z, dpre=dz)
+    leaf = z.double().requires_grad_(True)
+    ref, = torch.autograd.grad(act64_far(leaf, act).sum(), leaf)
+    check(dz, ref, rounded(ref, 2 * rel * ref.abs(), dt), "act'")
+
+
+def act64_far(z, name):
+    """act64 without tanh's cancellation: z sigmoid(z), z sigmoid(2 u)."""
+    return z * torch.sigmoid(z if name == "silu" else math.sqrt(8 / math.pi) * (z + 0.044715 * z ** 3))
