@@ -219,14 +219,15 @@ int product(const Product& p, const Epi& epi) {
 // column sums in registers.  They are added across the CTA's row lanes in
 // shared memory, then across the cluster in rank order over distributed shared
 // memory: a fixed order and no scratch in global memory.  dz may be dy or pre:
-// every element is read before it is written, by the same thread.
+// every element is read before it is written, by the same thread.  The
+// activation is a template parameter: chosen inside, the one-row form held to 32
+// registers spilled 16 to 44 bytes (4096 x 8192 SILU: 41.8 us against 37.7).
 constexpr uint32_t kDactCluster = 8;
 constexpr int kDactThreads = 256;
 
-template <typename T, int L, int U>
+template <typename T, int L, int U, int ACT>
 __global__ void __cluster_dims__(1, kDactCluster, 1) __launch_bounds__(kDactThreads, U == 1 ? 8 : 3)
-    dact_kernel(const T* dy, const T* pre, T* dz, T* dbias, uint32_t rows, uint32_t N, int act, int acc,
-                int trigger) {
+    dact_kernel(const T* dy, const T* pre, T* dz, T* dbias, uint32_t rows, uint32_t N, int acc, int trigger) {
     constexpr uint32_t RL = kDactThreads / L;  // row lanes
     __shared__ float s_sum[RL][8 * L + 1];
     __shared__ float s_col[8 * L];
@@ -242,22 +243,21 @@ __global__ void __cluster_dims__(1, kDactCluster, 1) __launch_bounds__(kDactThre
             Vec8 a[U], z[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                // past the end its first row again: others may be writing theirs (dz may be dy or pre).
-                // At U = 1 min is r, but the compiler spills less with it (4096 x 8192: 41.5 us, not 43.5).
-                const uint32_t row = U == 1 ? min(r, r1 - 1) : r + u * RL < r1 ? r + u * RL : r;
+                // past the end its first row again: others may be writing theirs (dz may be dy or pre)
+                const uint32_t row = U == 1 || r + u * RL < r1 ? r + u * RL : r;
                 const uint64_t at = (uint64_t)row * N + col;
                 a[u] = ld_vec8(dy + at);
-                if (act != EVKCU_ACT_NONE) z[u] = ld_vec8(pre + at);
+                if (ACT != EVKCU_ACT_NONE) z[u] = ld_vec8(pre + at);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (r + u * RL >= r1) break;
                 float f[8];
                 unpack8<T>(a[u], f);
-                if (act != EVKCU_ACT_NONE) {
+                if (ACT != EVKCU_ACT_NONE) {
                     float y[8];
                     unpack8<T>(z[u], y);
-                    dact_all(f, y, act);
+                    dact_all(f, y, ACT);
                     st_vec8(dz + (uint64_t)(r + u * RL) * N + col, pack8<T>(f));
                 }
 #pragma unroll
@@ -295,16 +295,26 @@ __global__ void __cluster_dims__(1, kDactCluster, 1) __launch_bounds__(kDactThre
 template <typename T, int L, int U>
 int launch_dact_of(const void* dy, const void* pre, void* dz, void* dbias, uint32_t rows, uint32_t N, int act, int acc,
                    int trigger, cudaStream_t st) {
-    return launch_pdl("evkcu_linear_backward(dact)", dact_kernel<T, L, U>,
-                      dim3((N + 8 * L - 1) / (8 * L), kDactCluster), dim3(kDactThreads), 0, st, (const T*)dy,
-                      (const T*)pre, (T*)dz, (T*)dbias, rows, N, act, acc, trigger);
+    auto go = [&](auto kern) {
+        return launch_pdl("evkcu_linear_backward(dact)", kern, dim3((N + 8 * L - 1) / (8 * L), kDactCluster),
+                          dim3(kDactThreads), 0, st, (const T*)dy, (const T*)pre, (T*)dz, (T*)dbias, rows, N, acc,
+                          trigger);
+    };
+    switch (act) {
+        case EVKCU_ACT_RELU: return go(dact_kernel<T, L, U, EVKCU_ACT_RELU>);
+        case EVKCU_ACT_GELU: return go(dact_kernel<T, L, U, EVKCU_ACT_GELU>);
+        case EVKCU_ACT_SILU: return go(dact_kernel<T, L, U, EVKCU_ACT_SILU>);
+        default: return go(dact_kernel<T, L, U, EVKCU_ACT_NONE>);
+    }
 }
 
 // One row a lane and eight CTAs an SM hide the memory best where there are
-// that many CTAs: 32 columns a cluster (4096 x 8192: 48 us; 64 columns 52,
-// four rows a lane and 64 columns 68), 16 in narrower layers (16384 x 2048:
-// 52 us against 63), and four rows a lane where even those are too few
-// (16384 x 512: 19 us against 28).
+// that many CTAs: 32 columns a cluster (4096 x 8192 GELU: 45 us; 64 columns 49,
+// four rows a lane and 64 columns 56), 16 in narrower layers (16384 x 2048: 49 us
+// against 57), and four rows a lane where even those are too few (16384 x 512:
+// 19 us against 26).  Set at GELU; SILU and RELU, which compute less, take 37,
+// 46 and 13 us there, and 64 columns would do in 35 (one row a lane) and, four rows
+// a lane, 39 us.
 template <typename T>
 int launch_dact(const void* dy, const void* pre, void* dz, void* dbias, uint32_t rows, uint32_t N, int act, int acc,
                 int trigger, cudaStream_t st) {
