@@ -503,6 +503,15 @@ def _same_ptrs(op, like, want):
     return out
 
 
+def _row_count(op, x, a, b):
+    """Rows of x's last dimension a.  The C ABI takes 32-bit sizes, and ctypes
+    would cut larger ones to their low bits."""
+    rows = x.numel() // a if a else 0
+    if (rows | a | b) >> 32:
+        raise EvkcuError(op, 1, f"{rows} rows of {a} and {b} columns: sizes above 2^32 - 1")
+    return rows
+
+
 def linear(x, w, y, bias=None, residual=None, act=ACT_NONE, pre=None, transpose_w=False, stream=None):
     """y = act(x @ w + bias) + residual (evkcu_linear).
 
@@ -512,10 +521,11 @@ def linear(x, w, y, bias=None, residual=None, act=ACT_NONE, pre=None, transpose_
     *lead, K = x.shape
     N = y.shape[-1]
     out = (*lead, N)
+    rows = _row_count("linear", x, K, N)
     p = _same_ptrs("linear", x, (("x", x, x.shape), ("w", w, (N, K) if transpose_w else (K, N)), ("bias", bias, (N,)),
                                  ("residual", residual, out), ("y", y, out), ("pre", pre, out)))
     _check("evkcu_linear", lib().evkcu_linear(
-        *p, x.numel() // K if K else 0, K, N, act, MM_TRANSPOSE_B if transpose_w else 0, _dtype_code(x),
+        *p, rows, K, N, act, MM_TRANSPOSE_B if transpose_w else 0, _dtype_code(x),
         _stream(stream)))
     return y
 
@@ -529,12 +539,13 @@ def linear_backward(x, w, dy, dx=None, dw=None, dbias=None, act=ACT_NONE, pre=No
     K, N = x.shape[-1], dy.shape[-1]
     out = (*x.shape[:-1], N)
     wshape = (N, K) if transpose_w else (K, N)
+    rows = _row_count("linear_backward", x, K, N)
     p = _same_ptrs("linear_backward", x, (("x", x, x.shape), ("w", w, wshape), ("pre", pre, out), ("dy", dy, out),
                                           ("dpre", dpre, out), ("dx", dx, x.shape), ("dw", dw, wshape),
                                           ("dbias", dbias, (N,))))
     flags = (MM_TRANSPOSE_B if transpose_w else 0) | (MM_ACC_C if acc else 0)
     _check("evkcu_linear_backward", lib().evkcu_linear_backward(
-        *p, x.numel() // K if K else 0, K, N, act, flags, _dtype_code(x), _stream(stream)))
+        *p, rows, K, N, act, flags, _dtype_code(x), _stream(stream)))
     return dx, dw, dbias
 
 
@@ -547,12 +558,13 @@ def gated_ffn(x, w_in, w_out, y, hidden, act=ACT_SILU, residual=None, pre=None, 
     gated_ffn_backward.  y = None (then w_out may be None) stops at hidden."""
     D, F = x.shape[-1], hidden.shape[-1]
     lead = x.shape[:-1]
+    rows = _row_count("gated_ffn", x, D, F)
     p = _same_ptrs("gated_ffn", x, (("x", x, x.shape), ("w_in", w_in, (2 * F, D) if transpose_w else (D, 2 * F)),
                                     ("w_out", w_out, (D, F) if transpose_w else (F, D)),
                                     ("residual", residual, x.shape), ("y", y, x.shape), ("hidden", hidden, (*lead, F)),
                                     ("pre", pre, (*lead, 2 * F))))
     _check("evkcu_gated_ffn", lib().evkcu_gated_ffn(
-        *p, x.numel() // D if D else 0, D, F, act, MM_TRANSPOSE_B if transpose_w else 0, _dtype_code(x),
+        *p, rows, D, F, act, MM_TRANSPOSE_B if transpose_w else 0, _dtype_code(x),
         _stream(stream)))
     return y if y is not None else hidden
 
@@ -565,6 +577,7 @@ def gated_ffn_backward(x, w_in, w_out, pre, dy, dpre, hidden, dx=None, dw_in=Non
     (..., F) is recomputed and needed only for dw_out."""
     D, F = x.shape[-1], pre.shape[-1] // 2
     lead = x.shape[:-1]
+    rows = _row_count("gated_ffn_backward", x, D, F)
     si, so = ((2 * F, D), (D, F)) if transpose_w else ((D, 2 * F), (F, D))
     p = _same_ptrs("gated_ffn_backward", x, (("x", x, x.shape), ("w_in", w_in, si), ("w_out", w_out, so),
                                              ("pre", pre, (*lead, 2 * F)), ("dy", dy, x.shape),
@@ -572,7 +585,7 @@ def gated_ffn_backward(x, w_in, w_out, pre, dy, dpre, hidden, dx=None, dw_in=Non
                                              ("dx", dx, x.shape), ("dw_in", dw_in, si), ("dw_out", dw_out, so)))
     flags = (MM_TRANSPOSE_B if transpose_w else 0) | (MM_ACC_C if acc else 0)
     _check("evkcu_gated_ffn_backward", lib().evkcu_gated_ffn_backward(
-        *p, x.numel() // D if D else 0, D, F, act, flags, _dtype_code(x), _stream(stream)))
+        *p, rows, D, F, act, flags, _dtype_code(x), _stream(stream)))
     return dx, dw_in, dw_out
 
 
@@ -596,6 +609,8 @@ def _qk_shape(op, q, k, heads, positions, rot_dim, pos_offset):
         if dh == 0 or k.dim() != 3 or k.shape[2] % dh:
             raise EvkcuError(op, 1, f"k is {tuple(k.shape)}, expected (B, S, kv_heads * {dh})")
         kc = k.shape[2]
+    if (B | S | cols | kc) >> 32:  # as in _row_count
+        raise EvkcuError(op, 1, f"q is {tuple(q.shape)}, with {kc} columns of keys: sizes above 2^32 - 1")
     pos = None
     if positions is not None:
         torch = _torch or _get_torch()
@@ -628,6 +643,8 @@ def qk_norm_rope(q, k, q_out, k_out, heads: int, gain_q=None, gain_k=None, v=Non
         if k_out.dim() != 3:
             raise EvkcuError(op, 1, f"k_out is {tuple(k_out.shape)}, expected (B, cache_len, {kc})")
         cache_len = k_out.shape[1]
+        if cache_len >> 32:
+            raise EvkcuError(op, 1, f"a cache of {cache_len} rows: sizes above 2^32 - 1")
     ks = (B, S, kc)
     os = (B, cache_len, kc) if cache else ks
     _same(op, q, (("q_out", q_out, q.shape), ("gain_q", gain_q, (dh,)), ("gain_k", gain_k, (dh,)), ("k", k, ks),

@@ -1,0 +1,45 @@
+"""Calls of the decoder-layer operators that the Python binding and the C++
+layer turn away before anything is computed; none needs a GPU."""
+import pytest
+import torch
+
+import evk_b200 as evk
+
+SHAPE, ARG = 1, 7
+BIG = 1 << 32
+
+
+def meta(*shape):
+    """A tensor of that shape and type without memory."""
+    return torch.empty(*shape, dtype=torch.float16, device="meta")
+
+
+def refused(status, f, *a, **kw):
+    with pytest.raises(evk.EvkcuError) as e:
+        f(*a, **kw)
+    assert e.value.status == status, e.value
+
+
+@pytest.mark.parametrize("rows,K,N", [(BIG, 8, 8), (BIG + 5, 8, 16), (1, BIG, 8), (1, 8, BIG), (3, 8, BIG + 8)])
+def test_sizes_past_32_bits_are_refused(rows, K, N):
+    """The C ABI takes 32-bit sizes; a call must not be cut to its low bits."""
+    x, w, y = meta(rows, K), meta(K, N), meta(rows, N)
+    refused(SHAPE, evk.linear, x, w, y)
+    refused(SHAPE, evk.linear, x.view(rows, 1, K), w, y.view(rows, 1, N))
+    refused(SHAPE, evk.linear_backward, x, w, y, dx=meta(rows, K))
+    refused(SHAPE, evk.gated_ffn, x, meta(K, 2 * N), meta(N, K), meta(rows, K), y)
+    refused(SHAPE, evk.gated_ffn_backward, x, meta(K, 2 * N), meta(N, K), meta(rows, 2 * N), meta(rows, K),
+            meta(rows, 2 * N), y, dx=meta(rows, K))
+
+
+@pytest.mark.parametrize("B,S,H,dh", [(BIG, 1, 1, 8), (1, BIG + 3, 1, 8), (1, 1, BIG, 8), (2, 1, BIG + 2, 8)])
+def test_qk_sizes_past_32_bits_are_refused(B, S, H, dh):
+    q = meta(B, S, H * dh)
+    refused(SHAPE, evk.qk_norm_rope, q, None, meta(B, S, H * dh), None, H)
+    refused(SHAPE, evk.qk_norm_rope_backward, q, None, q, None, meta(B, S, H * dh), None, H)
+
+
+def test_keys_and_caches_past_32_bits_are_refused():
+    q, k = meta(1, 1, 8), meta(1, 1, 8)
+    refused(SHAPE, evk.qk_norm_rope, q, meta(1, 1, 8 * BIG), meta(1, 1, 8), meta(1, 1, 8 * BIG), 1)
+    refused(SHAPE, evk.qk_norm_rope, q, k, meta(1, 1, 8), meta(1, BIG + 4, 8), 1, cache=True)
