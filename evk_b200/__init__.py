@@ -503,6 +503,13 @@ def _same_ptrs(op, like, want):
     return out
 
 
+def _missing(op, **tensors):
+    """The error of a call that lacks one of these tensors, from which the
+    binding takes shapes and strides (the C ABI checks the others)."""
+    names = ", ".join(n for n, t in tensors.items() if t is None)
+    return EvkcuError(op, 7, f"{names} must be given")
+
+
 def _row_count(op, x, a, b):
     """Rows of x's last dimension a.  The C ABI takes 32-bit sizes, and ctypes
     would cut larger ones to their low bits."""
@@ -518,6 +525,8 @@ def linear(x, w, y, bias=None, residual=None, act=ACT_NONE, pre=None, transpose_
     x (..., K); w (K, N), or (N, K) with transpose_w; bias (N,); residual, y
     and pre (..., N), pre receiving x @ w + bias for linear_backward.  residual
     may be y."""
+    if x is None or y is None:
+        raise _missing("linear", x=x, y=y)
     *lead, K = x.shape
     N = y.shape[-1]
     out = (*lead, N)
@@ -536,6 +545,8 @@ def linear_backward(x, w, dy, dx=None, dw=None, dbias=None, act=ACT_NONE, pre=No
     and dbias that are given; acc adds to them.  With an activation, pre is
     linear's and dpre (like pre; pre or dy itself is allowed) receives the
     gradient of x @ w + bias."""
+    if x is None or dy is None:
+        raise _missing("linear_backward", x=x, dy=dy)
     K, N = x.shape[-1], dy.shape[-1]
     out = (*x.shape[:-1], N)
     wshape = (N, K) if transpose_w else (K, N)
@@ -556,6 +567,8 @@ def gated_ffn(x, w_in, w_out, y, hidden, act=ACT_SILU, residual=None, pre=None, 
     x, y, residual (..., D); w_in (D, 2 F), w_out (F, D), or both transposed
     with transpose_w; hidden (..., F); pre (..., 2 F) receives [g | u] for
     gated_ffn_backward.  y = None (then w_out may be None) stops at hidden."""
+    if x is None or hidden is None:
+        raise _missing("gated_ffn", x=x, hidden=hidden)
     D, F = x.shape[-1], hidden.shape[-1]
     lead = x.shape[:-1]
     rows = _row_count("gated_ffn", x, D, F)
@@ -575,6 +588,8 @@ def gated_ffn_backward(x, w_in, w_out, pre, dy, dpre, hidden, dx=None, dw_in=Non
     dx, dw_in and dw_out that are given; acc adds to them.  pre is gated_ffn's;
     dpre (like pre; pre itself is allowed) receives its gradient; hidden
     (..., F) is recomputed and needed only for dw_out."""
+    if x is None or pre is None:
+        raise _missing("gated_ffn_backward", x=x, pre=pre)
     D, F = x.shape[-1], pre.shape[-1] // 2
     lead = x.shape[:-1]
     rows = _row_count("gated_ffn_backward", x, D, F)
@@ -634,6 +649,8 @@ def qk_norm_rope(q, k, q_out, k_out, heads: int, gain_q=None, gain_k=None, v=Non
     their positions.  v, where given, is copied along to v_out, which is laid
     out as k_out."""
     op = "qk_norm_rope"
+    if q is None or q_out is None or (k is not None and k_out is None):
+        raise _missing(op, q=q, q_out=q_out, **(dict(k_out=k_out) if k is not None else {}))
     B, S, dh, kc, pos = _qk_shape(op, q, k, heads, positions, rot_dim, pos_offset)
     cache_len = 0
     if k is None:
@@ -687,6 +704,8 @@ def qk_norm_rope_backward(q, k, dq_out, dk_out, dq, dk, heads: int, gain_q=None,
     `workspace` tensor of qk_norm_rope_workspace(Dh) bytes and are added to with
     acc_gain."""
     op = "qk_norm_rope_backward"
+    if q is None or dq_out is None or dq is None or (k is not None and (dk_out is None or dk is None)):
+        raise _missing(op, q=q, dq_out=dq_out, dq=dq, **(dict(dk_out=dk_out, dk=dk) if k is not None else {}))
     B, S, dh, kc, pos = _qk_shape(op, q, k, heads, positions, rot_dim, pos_offset)
     ks = (B, S, kc)
     if k is None:

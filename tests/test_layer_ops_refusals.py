@@ -43,3 +43,25 @@ def test_keys_and_caches_past_32_bits_are_refused():
     q, k = meta(1, 1, 8), meta(1, 1, 8)
     refused(SHAPE, evk.qk_norm_rope, q, meta(1, 1, 8 * BIG), meta(1, 1, 8), meta(1, 1, 8 * BIG), 1)
     refused(SHAPE, evk.qk_norm_rope, q, k, meta(1, 1, 8), meta(1, BIG + 4, 8), 1, cache=True)
+
+
+def test_missing_tensors_are_refused():
+    """None for a tensor that gives the binding a call's shapes: its error, with
+    a status (the others are refused by the C ABI)."""
+    t, w = meta(4, 8), meta(8, 8)
+    for n in ("x", "y"):
+        refused(ARG, evk.linear, **{**dict(x=t, w=w, y=t), n: None})
+    for n in ("x", "dy"):
+        refused(ARG, evk.linear_backward, **{**dict(x=t, w=w, dy=t), n: None})
+    for n in ("x", "hidden"):
+        refused(ARG, evk.gated_ffn, **{**dict(x=t, w_in=meta(8, 16), w_out=w, y=t, hidden=t), n: None})
+    back = dict(x=t, w_in=meta(8, 16), w_out=w, pre=meta(4, 16), dy=t, dpre=meta(4, 16), hidden=t)
+    for n in ("x", "pre"):
+        refused(ARG, evk.gated_ffn_backward, **{**back, n: None})
+    q = meta(1, 2, 16)
+    for n in ("q", "q_out", "k_out"):
+        refused(ARG, evk.qk_norm_rope, **{**dict(q=q, k=q, q_out=q, k_out=q, heads=2), n: None})
+    refused(ARG, evk.qk_norm_rope, q, q, q, None, 2, cache=True)
+    for n in ("q", "dq_out", "dq", "dk_out", "dk"):
+        refused(ARG, evk.qk_norm_rope_backward,
+                **{**dict(q=q, k=q, dq_out=q, dk_out=q, dq=q, dk=q, heads=2), n: None})
