@@ -85,6 +85,8 @@ using evk_b200::dptr;
 const void* opt(Tensor* t) { return t ? dptr(*t) : nullptr; }
 void* opt_mut(Tensor* t) { return t ? dmut(*t) : nullptr; }
 uint64_t count(Tensor& t) { return t.shape.count(); }
+// Rows of t's last dimension (0 where that is 0).
+uint64_t rows_of(Tensor& t) { return t.shape[-1] ? count(t) / t.shape[-1] : 0; }
 // Every optional tensor that is given holds n elements.
 bool sized(uint64_t n, std::initializer_list<Tensor*> ts) {
     for (Tensor* t : ts)
@@ -100,8 +102,8 @@ bool is_matrix(Tensor& t, uint64_t rows, uint64_t cols, bool transposed) {
 
 void linear(Tensor& x, Tensor& w, Tensor& y, Tensor* bias, Tensor* residual, Act act, Tensor* pre, bool transpose_w,
             DType d) {
-    const uint64_t K = x.shape[-1], N = y.shape[-1], rows = count(x) / K;
-    if (!is_matrix(w, K, N, transpose_w) || !sized(rows * N, {&y, residual, pre}) || !sized(N, {bias}))
+    const uint64_t K = x.shape[-1], N = y.shape[-1], rows = rows_of(x);
+    if (K == 0 || !is_matrix(w, K, N, transpose_w) || !sized(rows * N, {&y, residual, pre}) || !sized(N, {bias}))
         return be().fail(EVKCU_BAD_SHAPE, "linear: incompatible shapes");
     evk_b200::check(be(),
                     evkcu_linear(dptr(x), dptr(w), opt(bias), opt(residual), dmut(y), opt_mut(pre), (uint32_t)rows,
@@ -112,8 +114,8 @@ void linear(Tensor& x, Tensor& w, Tensor& y, Tensor* bias, Tensor* residual, Act
 
 void linear_backward(Tensor& x, Tensor& w, Tensor& dy, Tensor* dx, Tensor* dw, Tensor* dbias, Act act, Tensor* pre,
                      Tensor* dpre, bool transpose_w, bool acc, DType d) {
-    const uint64_t K = x.shape[-1], N = dy.shape[-1], rows = count(x) / K;
-    if (!is_matrix(w, K, N, transpose_w) || (dw && !is_matrix(*dw, K, N, transpose_w)) ||
+    const uint64_t K = x.shape[-1], N = dy.shape[-1], rows = rows_of(x);
+    if (K == 0 || !is_matrix(w, K, N, transpose_w) || (dw && !is_matrix(*dw, K, N, transpose_w)) ||
         !sized(rows * N, {&dy, pre, dpre}) || !sized(count(x), {dx}) || !sized(N, {dbias}))
         return be().fail(EVKCU_BAD_SHAPE, "linear_backward: incompatible shapes");
     const uint32_t flags = (transpose_w ? EVKCU_MM_TRANSPOSE_B : 0u) | (acc ? EVKCU_MM_ACC_C : 0u);
@@ -126,8 +128,8 @@ void linear_backward(Tensor& x, Tensor& w, Tensor& dy, Tensor* dx, Tensor* dw, T
 
 void gated_ffn(Tensor& x, Tensor& w_in, Tensor& w_out, Tensor& y, Tensor& hidden, Act act, Tensor* residual,
                Tensor* pre, bool transpose_w, DType d) {
-    const uint64_t D = x.shape[-1], F = hidden.shape[-1], rows = count(x) / D;
-    if (!is_matrix(w_in, D, 2 * F, transpose_w) || !is_matrix(w_out, F, D, transpose_w) ||
+    const uint64_t D = x.shape[-1], F = hidden.shape[-1], rows = rows_of(x);
+    if (D == 0 || !is_matrix(w_in, D, 2 * F, transpose_w) || !is_matrix(w_out, F, D, transpose_w) ||
         !sized(rows * D, {&y, residual}) || !sized(rows * F, {&hidden}) || !sized(2 * rows * F, {pre}))
         return be().fail(EVKCU_BAD_SHAPE, "gated_ffn: incompatible shapes");
     evk_b200::check(be(),
@@ -139,8 +141,8 @@ void gated_ffn(Tensor& x, Tensor& w_in, Tensor& w_out, Tensor& y, Tensor& hidden
 
 void gated_ffn_backward(Tensor& x, Tensor& w_in, Tensor& w_out, Tensor& pre, Tensor& dy, Tensor& dpre, Tensor& hidden,
                         Tensor* dx, Tensor* dw_in, Tensor* dw_out, Act act, bool transpose_w, bool acc, DType d) {
-    const uint64_t D = x.shape[-1], F = hidden.shape[-1], rows = count(x) / D;
-    if (!is_matrix(w_in, D, 2 * F, transpose_w) || !is_matrix(w_out, F, D, transpose_w) ||
+    const uint64_t D = x.shape[-1], F = hidden.shape[-1], rows = rows_of(x);
+    if (D == 0 || !is_matrix(w_in, D, 2 * F, transpose_w) || !is_matrix(w_out, F, D, transpose_w) ||
         (dw_in && !is_matrix(*dw_in, D, 2 * F, transpose_w)) || (dw_out && !is_matrix(*dw_out, F, D, transpose_w)) ||
         !sized(rows * D, {&dy, dx}) || !sized(rows * F, {&hidden}) || !sized(2 * rows * F, {&pre, &dpre}))
         return be().fail(EVKCU_BAD_SHAPE, "gated_ffn_backward: incompatible shapes");

@@ -1,9 +1,14 @@
 """Calls of the decoder-layer operators that the Python binding and the C++
 layer turn away before anything is computed; none needs a GPU."""
+import os
+import signal
+import subprocess
+
 import pytest
 import torch
 
 import evk_b200 as evk
+from conftest import ROOT
 
 SHAPE, ARG = 1, 7
 BIG = 1 << 32
@@ -65,3 +70,16 @@ def test_missing_tensors_are_refused():
     for n in ("q", "dq_out", "dq", "dk_out", "dk"):
         refused(ARG, evk.qk_norm_rope_backward,
                 **{**dict(q=q, k=q, dq_out=q, dk_out=q, dq=q, dk=q, heads=2), n: None})
+
+
+REFUSALS = os.path.join(ROOT, "evk_b200", "reftests", "layer_refusals")
+
+
+@pytest.mark.skipif(not os.path.exists(REFUSALS), reason="layer_refusals not built")
+@pytest.mark.parametrize("case", ["linear of nothing", "linear_backward of nothing", "gated_ffn of nothing",
+                                  "gated_ffn_backward of nothing"])
+def test_cpp_layer_refuses(case):
+    """The C++ layer's refusal: its message with EVKCU_BAD_SHAPE, then abort."""
+    r = subprocess.run([REFUSALS, case], capture_output=True, text=True, timeout=120)
+    assert r.returncode == -signal.SIGABRT, (r.returncode, r.stdout, r.stderr)
+    assert f"evk::ai::{case.split()[0]}" in r.stderr and "failed (status 1)" in r.stderr
