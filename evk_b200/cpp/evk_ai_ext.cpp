@@ -2,6 +2,7 @@
 // same shape logic (evk_ai_dispatch.h) and backend table as evk_ai.cpp.
 #include "evk_ai_ext.h"
 
+#include <algorithm>
 #include <cmath>
 #include <initializer_list>
 
@@ -84,17 +85,24 @@ using evk_b200::dptr;
 
 const void* opt(Tensor* t) { return t ? dptr(*t) : nullptr; }
 void* opt_mut(Tensor* t) { return t ? dmut(*t) : nullptr; }
-uint64_t count(Tensor& t) { return t.shape.count(); }
+// Elements of t, 2^32 for all that do not fit 32 bits: Shape::count(), by which
+// buffers are allocated, keeps only those.
+uint64_t count(Tensor& t) {
+    uint64_t n = 1;
+    for (uint32_t i = 0; i < t.shape.rank(); ++i) n = std::min(n * t.shape[(int)i], uint64_t(1) << 32);
+    return n;
+}
+bool fits(Tensor& t) { return count(t) >> 32 == 0; }
 // Rows of t's last dimension (0 where that is 0).
 uint64_t rows_of(Tensor& t) { return t.shape[-1] ? count(t) / t.shape[-1] : 0; }
 // Every optional tensor that is given holds n elements.
 bool sized(uint64_t n, std::initializer_list<Tensor*> ts) {
     for (Tensor* t : ts)
-        if (t && count(*t) != n) return false;
+        if (t && (!fits(*t) || count(*t) != n)) return false;
     return true;
 }
 bool is_matrix(Tensor& t, uint64_t rows, uint64_t cols, bool transposed) {
-    if (t.shape.rank() != 2) return false;
+    if (t.shape.rank() != 2 || !fits(t)) return false;
     return t.shape[0] == (transposed ? cols : rows) && t.shape[1] == (transposed ? rows : cols);
 }
 
@@ -103,7 +111,8 @@ bool is_matrix(Tensor& t, uint64_t rows, uint64_t cols, bool transposed) {
 void linear(Tensor& x, Tensor& w, Tensor& y, Tensor* bias, Tensor* residual, Act act, Tensor* pre, bool transpose_w,
             DType d) {
     const uint64_t K = x.shape[-1], N = y.shape[-1], rows = rows_of(x);
-    if (K == 0 || !is_matrix(w, K, N, transpose_w) || !sized(rows * N, {&y, residual, pre}) || !sized(N, {bias}))
+    if (K == 0 || !fits(x) || !is_matrix(w, K, N, transpose_w) || !sized(rows * N, {&y, residual, pre}) ||
+        !sized(N, {bias}))
         return be().fail(EVKCU_BAD_SHAPE, "linear: incompatible shapes");
     evk_b200::check(be(),
                     evkcu_linear(dptr(x), dptr(w), opt(bias), opt(residual), dmut(y), opt_mut(pre), (uint32_t)rows,
@@ -115,7 +124,7 @@ void linear(Tensor& x, Tensor& w, Tensor& y, Tensor* bias, Tensor* residual, Act
 void linear_backward(Tensor& x, Tensor& w, Tensor& dy, Tensor* dx, Tensor* dw, Tensor* dbias, Act act, Tensor* pre,
                      Tensor* dpre, bool transpose_w, bool acc, DType d) {
     const uint64_t K = x.shape[-1], N = dy.shape[-1], rows = rows_of(x);
-    if (K == 0 || !is_matrix(w, K, N, transpose_w) || (dw && !is_matrix(*dw, K, N, transpose_w)) ||
+    if (K == 0 || !fits(x) || !is_matrix(w, K, N, transpose_w) || (dw && !is_matrix(*dw, K, N, transpose_w)) ||
         !sized(rows * N, {&dy, pre, dpre}) || !sized(count(x), {dx}) || !sized(N, {dbias}))
         return be().fail(EVKCU_BAD_SHAPE, "linear_backward: incompatible shapes");
     const uint32_t flags = (transpose_w ? EVKCU_MM_TRANSPOSE_B : 0u) | (acc ? EVKCU_MM_ACC_C : 0u);
@@ -129,7 +138,7 @@ void linear_backward(Tensor& x, Tensor& w, Tensor& dy, Tensor* dx, Tensor* dw, T
 void gated_ffn(Tensor& x, Tensor& w_in, Tensor& w_out, Tensor& y, Tensor& hidden, Act act, Tensor* residual,
                Tensor* pre, bool transpose_w, DType d) {
     const uint64_t D = x.shape[-1], F = hidden.shape[-1], rows = rows_of(x);
-    if (D == 0 || !is_matrix(w_in, D, 2 * F, transpose_w) || !is_matrix(w_out, F, D, transpose_w) ||
+    if (D == 0 || !fits(x) || !is_matrix(w_in, D, 2 * F, transpose_w) || !is_matrix(w_out, F, D, transpose_w) ||
         !sized(rows * D, {&y, residual}) || !sized(rows * F, {&hidden}) || !sized(2 * rows * F, {pre}))
         return be().fail(EVKCU_BAD_SHAPE, "gated_ffn: incompatible shapes");
     evk_b200::check(be(),
@@ -142,7 +151,7 @@ void gated_ffn(Tensor& x, Tensor& w_in, Tensor& w_out, Tensor& y, Tensor& hidden
 void gated_ffn_backward(Tensor& x, Tensor& w_in, Tensor& w_out, Tensor& pre, Tensor& dy, Tensor& dpre, Tensor& hidden,
                         Tensor* dx, Tensor* dw_in, Tensor* dw_out, Act act, bool transpose_w, bool acc, DType d) {
     const uint64_t D = x.shape[-1], F = hidden.shape[-1], rows = rows_of(x);
-    if (D == 0 || !is_matrix(w_in, D, 2 * F, transpose_w) || !is_matrix(w_out, F, D, transpose_w) ||
+    if (D == 0 || !fits(x) || !is_matrix(w_in, D, 2 * F, transpose_w) || !is_matrix(w_out, F, D, transpose_w) ||
         (dw_in && !is_matrix(*dw_in, D, 2 * F, transpose_w)) || (dw_out && !is_matrix(*dw_out, F, D, transpose_w)) ||
         !sized(rows * D, {&dy, dx}) || !sized(rows * F, {&hidden}) || !sized(2 * rows * F, {&pre, &dpre}))
         return be().fail(EVKCU_BAD_SHAPE, "gated_ffn_backward: incompatible shapes");
@@ -162,7 +171,8 @@ bool qk_desc(evkcu_qk_norm_rope_desc& d, Tensor& qkv, Tensor& q, Tensor& k, Tens
              const QkRope& r) {
     if (qkv.shape.rank() != 3 || q.shape.rank() != 3 || k.shape.rank() != 3 || r.heads == 0 ||
         q.shape[2] % r.heads != 0 || q.shape[0] != qkv.shape[0] || q.shape[1] != qkv.shape[1] ||
-        k.shape[0] != qkv.shape[0] || qkv.shape[2] != q.shape[2] + 2 * k.shape[2])
+        k.shape[0] != qkv.shape[0] || qkv.shape[2] != q.shape[2] + 2 * (uint64_t)k.shape[2] || !fits(qkv) ||
+        !fits(q) || !fits(k))
         return false;
     const uint32_t Dh = q.shape[2] / r.heads;
     if (Dh == 0 || k.shape[2] % Dh != 0 || !sized(Dh, {gain_q, gain_k})) return false;
@@ -201,7 +211,7 @@ void qk_norm_rope_backward(Tensor& qkv, Tensor& dq, Tensor& dk, Tensor& dqkv, Te
                            Tensor* dgain_q, Tensor* dgain_k, Tensor* workspace, const QkRope& rope, DType d) {
     evkcu_qk_norm_rope_desc desc;
     if (!qk_desc(desc, qkv, dq, dk, gain_q, gain_k, rope) || !evk_b200::same_shape(qkv, dqkv) ||
-        dk.shape[1] != qkv.shape[1] || !sized(desc.head_dim, {dgain_q, dgain_k}))
+        dk.shape[1] != qkv.shape[1] || !sized(desc.head_dim, {dgain_q, dgain_k}) || (workspace && !fits(*workspace)))
         return be().fail(EVKCU_BAD_SHAPE, "qk_norm_rope_backward: incompatible shapes");
     const void* in = dptr(qkv);
     void* out = dmut(dqkv);

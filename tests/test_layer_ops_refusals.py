@@ -77,7 +77,10 @@ REFUSALS = os.path.join(ROOT, "evk_b200", "reftests", "layer_refusals")
 
 @pytest.mark.skipif(not os.path.exists(REFUSALS), reason="layer_refusals not built")
 @pytest.mark.parametrize("case", ["linear of nothing", "linear_backward of nothing", "gated_ffn of nothing",
-                                  "gated_ffn_backward of nothing"])
+                                  "gated_ffn_backward of nothing", "linear past 32 bits",
+                                  "linear_backward past 32 bits", "gated_ffn past 32 bits",
+                                  "gated_ffn_backward past 32 bits", "qk_norm_rope past 32 bits",
+                                  "qk_norm_rope_backward past 32 bits"])
 def test_cpp_layer_refuses(case):
     """The C++ layer's refusal: its message with EVKCU_BAD_SHAPE, then abort."""
     r = subprocess.run([REFUSALS, case], capture_output=True, text=True, timeout=120)
