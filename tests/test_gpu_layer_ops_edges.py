@@ -6,8 +6,8 @@ import pytest
 import torch
 
 import evk_b200 as evk
-from test_gpu_layer_ops import (ACTS, DTYPES, back_ref, check, ffn_back_ref, gen, lin_ref, qk_ref, qk_unit, rnd,
-                                rounded)
+from test_gpu_layer_ops import (ACTS, DTYPES, _layer, _layer_state, act64, back_ref, check, ffn_back_ref, gen, lin_ref,
+                                qk_ref, qk_unit, rnd, rounded)
 
 pytestmark = pytest.mark.gpu
 
@@ -207,3 +207,53 @@ def test_activations_of_far_negative_values(act, dt):
 def act64_far(z, name):
     """act64 without tanh's cancellation: z sigmoid(z), z sigmoid(2 u)."""
     return z * torch.sigmoid(z if name == "silu" else math.sqrt(8 / math.pi) * (z + 0.044715 * z ** 3))
+
+
+# ------------------------------------------------------------------ together --
+def layer_ref(s, H, Hk, dh, dt=None, leave_out=()):
+    """The decoder layer of test_gpu_layer_ops.py in 64 bits: as it is, with
+    every stored tensor (and the attention's weights) rounded to dt, or without
+    some of its parts."""
+    w = {n: t.double() for n, t in s.items()}
+    for n in ("gq", "gk"):
+        if n in leave_out:
+            w[n] = torch.ones_like(w[n])
+    r = (lambda t: t.to(dt).double()) if dt else (lambda t: t)
+    norm = lambda t: t * torch.rsqrt((t * t).mean(-1, keepdim=True) + 1e-5)  # noqa: E731
+    x = w["x"]
+    B, S, D = x.shape
+    pos = torch.arange(S, device="cuda")[None].expand(B, S) * (0 if "rotation" in leave_out else 1)
+    qkv = r(r(norm(x)) @ w["wqkv"] + (0 if "bias" in leave_out else w["bqkv"]))
+    q, k, v = qkv.split([H * dh, Hk * dh, Hk * dh], -1)
+    q = r(qk_ref(q, H, w["gq"], pos, 0, False, 10000.0, 1e-5)[0]).transpose(1, 2)
+    k = r(qk_ref(k, Hk, w["gk"], pos, 0, False, 10000.0, 1e-5)[0]).transpose(1, 2).repeat_interleave(H // Hk, 1)
+    v = v.reshape(B, S, Hk, dh).transpose(1, 2).repeat_interleave(H // Hk, 1)
+    sc = (q @ k.transpose(2, 3)) / math.sqrt(dh)
+    sc = sc.masked_fill(torch.ones(S, S, dtype=torch.bool, device="cuda").triu(1), -math.inf)
+    att = r((r(torch.softmax(sc, -1)) @ v).transpose(1, 2).reshape(B, S, D))
+    x1 = r(att @ w["wo"] + (0 if "first residual" in leave_out else x))
+    p = r(norm(x1)) @ w["wi"]
+    F = p.shape[-1] // 2
+    h = r((p[..., :F] if "activation" in leave_out else act64(p[..., :F], "silu")) * p[..., F:])
+    return r(h @ w["wd"] + (0 if "second residual" in leave_out else x1))
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_decoder_layer_would_show_a_missing_part(dt):
+    """The layer with gains and a bias that matter.  e is what rounding every
+    stored tensor does to the 64-bit layer; the kernels round the same tensors,
+    and their fp32 sums add little (K 2^-23 against 2^-11), so 3 e bounds them
+    in the 2-norm.  Leaving any part out moves the result by 6 e at least."""
+    B, S, H, Hk, dh, F = 2, 192, 8, 2, 64, 1368
+    s = _layer_state(dt, B, S, H, Hk, dh, F, 4)
+    g = gen(5)
+    s["gq"], s["gk"] = (rnd(g, dt, dh, std=0.5, mean=1.0) for _ in range(2))
+    s["bqkv"], s["wo"] = rnd(g, dt, (H + 2 * Hk) * dh, std=0.5), rnd(g, dt, H * dh, H * dh, std=2 * (H * dh) ** -0.5)
+    y = _layer(s, H, Hk, dh).double()
+    evk.check_device_error()
+    ref = layer_ref(s, H, Hk, dh)
+    far = lambda t: float((t - ref).norm())  # noqa: E731
+    e = far(layer_ref(s, H, Hk, dh, dt))
+    assert far(y) <= 3 * e, (far(y), e)
+    for part in ("gq", "gk", "rotation", "bias", "first residual", "second residual", "activation"):
+        assert far(layer_ref(s, H, Hk, dh, leave_out=(part,))) >= 6 * e, part
