@@ -644,10 +644,13 @@ def qk_norm_rope(q, k, q_out, k_out, heads: int, gain_q=None, gain_k=None, v=Non
 
     q, q_out (B, S, heads * Dh); k, k_out (B, S, Hkv * Dh), or None for queries
     only; rows may be slices of a fused QKV tensor.  gain_q, gain_k (Dh,).
-    positions: B * S int32 values, else pos_offset + t.  With cache=True, k_out
-    is a contiguous KV cache (B, cache_len, Hkv * Dh) and keys go to the rows of
-    their positions.  v, where given, is copied along to v_out, which is laid
-    out as k_out."""
+    rot_dim: the rotated part of a head, even, 0 for all of it; pairs are
+    (2 i, 2 i + 1), or (i, i + rot_dim / 2) with half_split, where the rotated
+    part (Dh, if rot_dim is 0) has to be a multiple of 16.  positions: B * S
+    int32 values, else pos_offset + t.  With cache=True, k_out is a contiguous
+    KV cache (B, cache_len, Hkv * Dh) and keys go to the rows of their
+    positions.  v, where given, is copied along to v_out, which is laid out as
+    k_out."""
     op = "qk_norm_rope"
     if q is None or q_out is None or (k is not None and k_out is None):
         raise _missing(op, q=q, q_out=q_out, **(dict(k_out=k_out) if k is not None else {}))

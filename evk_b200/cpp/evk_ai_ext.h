@@ -58,7 +58,8 @@ void greedy_sample_ex(Tensor& logits, Tensor& out_tokens, uint32_t position, uin
 
 // ---- decoder-layer operators around attention -------------------------------
 // The rules of include/evkcu.h hold (sizes in multiples of 8, which buffers
-// may coincide); optional tensors are pointers, nullptr for none.
+// may coincide), and a tensor holds less than 2^32 elements; optional tensors are
+// pointers, nullptr for none.
 enum class Act : int { None = 0, Relu = 1, Gelu = 2, Silu = 3 };
 
 // y = act(x w + bias) + residual over the rows of x's last dimension; w is
@@ -86,9 +87,11 @@ void gated_ffn_backward(Tensor& x, Tensor& w_in, Tensor& w_out, Tensor& pre, Ten
 // What qk_norm_rope rotates by, and how.
 struct QkRope {
     uint32_t heads = 0;
-    uint32_t rot_dim = 0;     // rotated part of a head, 0 for all of it
-    bool half_split = false;  // pairs (i, i + rot_dim / 2) instead of (2 i, 2 i + 1)
-    uint32_t pos_offset = 0;  // position of token t: pos_offset + t
+    uint32_t rot_dim = 0;     // rotated part of a head, even; 0 for all of it
+    bool half_split = false;  // pairs (i, i + rot_dim / 2) instead of (2 i, 2 i + 1); the
+                              // rotated part is then a multiple of 16
+    uint32_t pos_offset = 0;  // position of token t of every sequence: pos_offset + t
+                              // (positions of each sequence's own: evkcu_qk_norm_rope)
     float eps = 1e-5f, base = 10000.0f;
 };
 

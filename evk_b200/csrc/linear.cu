@@ -12,6 +12,13 @@
 // linear.cuh, in the paired-SM kernel (linear_pair.cuh) or the slab kernel
 // (linear_slab.cuh).  Transposed operands are MN-major descriptors, never
 // copies.
+//
+// Rounded to the storage type in between: dz, h and dpre, which are operands of
+// the next product, and the tensor cores take no wider ones at this rate (two
+// halves of a value would double that product).  The error of a result of theirs
+// is about sqrt(2) times that of its own rounding: 2-norm against 64 bits in bf16
+// 0.0023 to 0.0024 for y of one token and for the gradients, 0.0017 for one
+// rounding.  dh and the sums behind dbias are not rounded.
 #include <algorithm>
 #include <atomic>
 #include <cmath>

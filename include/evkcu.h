@@ -64,7 +64,8 @@ typedef enum evkcu_act {
 } evkcu_act;
 
 /* evkcu_qk_norm_rope flags */
-#define EVKCU_QK_HALF_SPLIT 1u /* pairs (i, i + rot_dim / 2) instead of (2 i, 2 i + 1) */
+#define EVKCU_QK_HALF_SPLIT 1u /* pairs (i, i + rot_dim / 2) instead of (2 i, 2 i + 1);
+                                  the rotated part is then a multiple of 16           */
 #define EVKCU_QK_CACHE 2u      /* keys and values go to their rows of a KV cache       */
 #define EVKCU_QK_ACC_GAIN 4u   /* backward: dgain += instead of =                      */
 
@@ -299,8 +300,8 @@ int evkcu_flash_attention_bwd(const void* q, const void* k, const void* v, const
  * No counterparts in the reference, whose layers compose matmul, gelu, add,
  * rms_norm and rope (example/main_llm.cpp:528-546).  Shared rules:
  *   - matrices are contiguous, 16-byte aligned; K, N, D and F are positive
- *     multiples of 8; any number of rows, 0 included (then the gradients of
- *     the weights and the bias are 0);
+ *     multiples of 8; rows, K, N, D and 2 F are at most 2^30, rows may be 0
+ *     (then the gradients of the weights and the bias are 0);
  *   - products accumulate in fp32 and every output is rounded once.  Tensors
  *     that the call itself reads back (dpre, hidden) are rounded to the
  *     storage type in between, as tensor-core operands have to be;
@@ -357,9 +358,12 @@ int evkcu_gated_ffn_backward(const void* x, const void* w_in, const void* w_out,
  * multiples of 8), so slices of a fused QKV projection are taken as they lie.
  * The position of a row is positions[r], or pos_offset + t without positions. */
 typedef struct evkcu_qk_norm_rope_desc {
-    uint32_t batch, seq_len, heads, kv_heads; /* kv_heads = 0: queries only           */
+    uint32_t batch, seq_len, heads, kv_heads; /* at most 2^30 rows, 65535 heads each;
+                                                 kv_heads = 0: queries only           */
     uint32_t head_dim;                        /* a multiple of 8, 8 to 256            */
-    uint32_t rot_dim;                         /* rotated part of a head; 0: all of it */
+    uint32_t rot_dim;                         /* rotated part of a head, even; 0: all of
+                                                 it.  With EVKCU_QK_HALF_SPLIT it (the
+                                                 head, where 0) is a multiple of 16   */
     uint32_t flags, pos_offset;
     uint32_t cache_len; /* EVKCU_QK_CACHE: rows of each sequence's cache              */
     float eps, base;
