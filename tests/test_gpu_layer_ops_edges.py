@@ -1,6 +1,7 @@
 """Edges of evkcu_linear, evkcu_gated_ffn and evkcu_qk_norm_rope that
 test_gpu_layer_ops.py does not reach, with its helpers and bounds."""
 import math
+import threading
 
 import pytest
 import torch
@@ -257,3 +258,48 @@ def test_decoder_layer_would_show_a_missing_part(dt):
     assert far(y) <= 3 * e, (far(y), e)
     for part in ("gq", "gk", "rotation", "bias", "first residual", "second residual", "activation"):
         assert far(layer_ref(s, H, Hk, dh, leave_out=(part,))) >= 6 * e, part
+
+
+def test_calls_from_threads_of_their_own():
+    """Host threads whose first CUDA call is an operator's, all at once: no
+    refusal, and the bits of calls from the main thread."""
+    dt, K, N = torch.bfloat16, 264, 520
+    sets = []
+    for rows in (1, 40, 130, 1030):
+        g = gen(rows)
+        x, w, wi, wo = rnd(g, dt, rows, K), rnd(g, dt, K, N), rnd(g, dt, K, 2 * N, std=0.1), rnd(g, dt, N, K, std=0.1)
+        dy, q = rnd(g, dt, rows, N), rnd(g, dt, 1, rows, 128)
+        e = lambda t: torch.empty_like(t)  # noqa: E731
+        sets.append((x, w, wi, wo, dy, q, e(dy), e(x), e(w), e(x), e(dy), e(q), torch.cuda.Stream()))
+
+    def work(x, w, wi, wo, dy, q, y, dx, dw, z, h, qo, stream):
+        evk.linear(x, w, y, act=evk.ACT_SILU, stream=stream)
+        evk.linear_backward(x, w, dy, dx=dx, dw=dw, stream=stream)
+        evk.gated_ffn(x, wi, wo, z, h, stream=stream)
+        evk.qk_norm_rope(q, None, qo, None, 2, stream=stream)
+        stream.synchronize()
+        return [t.clone() for t in (y, dx, dw, z, h, qo)]
+
+    want = [work(*s) for s in sets]
+    for s in sets:
+        for t in s[6:12]:
+            t.fill_(3.0)
+    torch.cuda.synchronize()
+    errors = []
+
+    def thread(s):
+        try:
+            for _ in range(10):
+                work(*s)
+        except Exception as e:  # noqa: BLE001 - shown by the assertion below
+            errors.append(e)
+
+    threads = [threading.Thread(target=thread, args=(s,)) for s in sets]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    torch.cuda.synchronize()
+    for s, w in zip(sets, want):
+        assert all(torch.equal(a, b) for a, b in zip(s[6:12], w))
